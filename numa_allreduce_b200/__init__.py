@@ -20,6 +20,12 @@ Public API (parity with the reference's ``src/__init__.py``, which exported
   :func:`pack_weight`, :func:`interleave_gate_up`: the tcgen05 GEMM and its
   fusions (SwiGLU epilogue; row-parallel GEMM -> allreduce -> residual ->
   RMSNorm);
+* :func:`assign_pages`, :func:`rope_append_paged`, :func:`paged_attention`,
+  :func:`rope_tables`: decode over a paged KV cache (block tables and slots on
+  the GPU, head norm + rotation + append, split attention for requests of
+  different lengths);
+* :func:`token_logprobs`, :func:`join_token_logprobs`: log-probabilities of
+  given tokens with entropy and top alternatives, per vocabulary shard;
 * :class:`LlamaConfig`, :class:`LlamaTPDecoder`: the tensor-parallel decoder
   built on them (in ``numa_allreduce_b200.models``, imported lazily);
 * :class:`PeerMonitor`, :class:`PeerLost`: host-side failure detection;
@@ -30,6 +36,8 @@ Public API (parity with the reference's ``src/__init__.py``, which exported
 from .ops.errors import KernelError, check_kernels, reset_kernels
 from .ops.fused import fused_allreduce_rmsnorm, rmsnorm_residual
 from .ops.gemm import PackedWeight, gemm, gemm_allreduce_rmsnorm, gemm_swiglu, interleave_gate_up, pack_weight
+from .ops.logprobs import TokenLogprobs, join_token_logprobs, token_logprobs
+from .ops.paged import PageSlots, assign_pages, paged_attention, rope_append_paged, rope_tables
 from .parallel.comm import AllReduceError, NumaAwareAllReduce
 from .parallel.emulate import emulate_all_gather, emulate_allreduce, emulate_reduce_scatter
 from .parallel.health import PeerLost, PeerMonitor
@@ -47,8 +55,11 @@ __all__ = [
     "NumaNodeInfo",
     "NumaTopology",
     "PackedWeight",
+    "PageSlots",
     "PeerLost",
     "PeerMonitor",
+    "TokenLogprobs",
+    "assign_pages",
     "check_kernels",
     "detect_numa_topology",
     "emulate_all_gather",
@@ -59,12 +70,17 @@ __all__ = [
     "gemm_allreduce_rmsnorm",
     "gemm_swiglu",
     "interleave_gate_up",
+    "join_token_logprobs",
     "pack_weight",
+    "paged_attention",
     "reference_all_gather",
     "reference_allreduce",
     "reference_reduce_scatter",
     "reset_kernels",
     "rmsnorm_residual",
+    "rope_append_paged",
+    "rope_tables",
+    "token_logprobs",
 ]
 
 __version__ = "0.1.0"

@@ -1,0 +1,302 @@
+// Torch bindings of the paged-cache decode operators and the token
+// log-probabilities. They are registered for every backend, so that a bad
+// argument is refused with its name whatever device it lies on; tensors on a
+// device other than CUDA are refused last.
+#include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+#include <torch/torch.h>
+
+#include <climits>
+#include <initializer_list>
+#include <optional>
+#include <tuple>
+#include <utility>
+
+#include "nab_common.h"
+#include "nab_logprobs.h"
+#include "nab_paged.h"
+
+namespace {
+
+using OptTensor = std::optional<at::Tensor>;
+using Named = std::pair<const char*, const at::Tensor*>;
+
+// The last check of every op: one CUDA device for all, and no gradients asked for.
+void check_devices(const char* op, std::initializer_list<Named> tensors) {
+  const at::Tensor& first = *tensors.begin()->second;
+  for (const auto& [name, t] : tensors) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), op, ": ", name,
+                " requires a gradient; this operator has none (use torch.no_grad())");
+    TORCH_CHECK(t->is_cuda(), op, ": ", name, " must be a CUDA tensor");
+    TORCH_CHECK(t->device() == first.device(), op, ": ", name, " is on ", t->device(), ", ", tensors.begin()->first,
+                " on ", first.device());
+  }
+}
+
+void check_vector(const char* op, const char* name, const at::Tensor& t, at::ScalarType type, int64_t n) {
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.scalar_type() == type, op, ": ", name,
+              " must be a contiguous ", type, " tensor of ", n, " elements");
+}
+
+int half_dtype(const char* op, const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name,
+              " must be bfloat16 or float16, got ", t.scalar_type());
+  return t.scalar_type() == at::kHalf ? nab::kF16 : nab::kBF16;
+}
+
+bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+// k_pages and v_pages: [pages, kv heads, P, D]
+void check_pages(const char* op, const at::Tensor& k, const at::Tensor& v, at::ScalarType type) {
+  TORCH_CHECK(k.dim() == 4 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes(), op,
+              ": k_pages and v_pages must be contiguous [pages, kv_heads, page_size, head_dim] of one shape");
+  TORCH_CHECK(k.scalar_type() == type && v.scalar_type() == type, op, ": k_pages and v_pages must be ", type);
+  TORCH_CHECK(k.size(0) >= 1 && k.size(1) >= 1, op, ": no pages");
+  TORCH_CHECK(k.size(2) >= 16 && k.size(2) % 16 == 0, op, ": page_size must be a multiple of 16, got ", k.size(2));
+  TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, op, ": head_dim must be 64 or 128, got ", k.size(3));
+  TORCH_CHECK(k.size(0) * k.size(1) * k.size(2) < INT_MAX, op, ": too many page rows");
+  TORCH_CHECK(aligned16(k) && aligned16(v), op, ": k_pages and v_pages must be 16-byte aligned");
+  if (k.is_cuda()) at::assert_no_overlap(k, v);
+}
+
+int sms_of(const at::Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at::Tensor& cached,
+                                                                        const OptTensor& query_start,
+                                                                        at::Tensor& block_tables,
+                                                                        const at::Tensor& free_pages,
+                                                                        const at::Tensor& taken, int64_t page_size,
+                                                                        int64_t num_tokens) {
+  constexpr const char* op = "assign_pages";
+  TORCH_CHECK(cached.dim() == 1 && cached.size(0) >= 1 && cached.size(0) <= nab::kMaxPagedRequests, op,
+              ": cached must hold 1 to ", nab::kMaxPagedRequests, " requests");
+  const int64_t B = cached.size(0);
+  check_vector(op, "cached", cached, at::kInt, B);
+  if (query_start) check_vector(op, "query_start", *query_start, at::kInt, B + 1);
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == B && block_tables.scalar_type() == at::kInt &&
+                  (block_tables.size(1) <= 1 || block_tables.stride(1) == 1) &&
+                  (B == 1 || block_tables.stride(0) >= block_tables.size(1)),
+              op, ": block_tables must be int32 [", B, ", pages], each row contiguous and apart from the others");
+  TORCH_CHECK(block_tables.size(1) * B < INT_MAX, op, ": block_tables is too large");
+  TORCH_CHECK(free_pages.dim() == 1 && free_pages.is_contiguous() && free_pages.scalar_type() == at::kInt &&
+                  free_pages.size(0) < INT_MAX,
+              op, ": free_pages must be a contiguous int32 vector");
+  check_vector(op, "taken", taken, at::kInt, 1);
+  TORCH_CHECK(page_size >= 16 && page_size % 16 == 0 && page_size <= (1 << 20), op,
+              ": page_size must be a multiple of 16, got ", page_size);
+  TORCH_CHECK(num_tokens >= 0 && num_tokens < INT_MAX, op, ": bad num_tokens ", num_tokens);
+  TORCH_CHECK(query_start || num_tokens >= B, op, ": num_tokens must be at least the ", B, " requests");
+  check_devices(op, {{"cached", &cached},
+                     {"query_start", query_start ? &*query_start : nullptr},
+                     {"block_tables", &block_tables},
+                     {"free_pages", &free_pages},
+                     {"taken", &taken}});
+  at::assert_no_overlap(block_tables, cached);
+  at::assert_no_overlap(block_tables, free_pages);
+  const at::cuda::CUDAGuard guard(cached.device());
+  at::Tensor positions = at::empty({num_tokens}, cached.options());
+  at::Tensor slots = at::empty({num_tokens}, cached.options().dtype(at::kLong));
+  at::Tensor lengths = at::empty({B}, cached.options());
+  at::Tensor taken_out = at::empty({1}, cached.options());
+  nab::AssignPagesArgs a{};
+  a.cached = cached.const_data_ptr<int>();
+  a.starts = query_start ? query_start->const_data_ptr<int>() : nullptr;
+  a.tables = block_tables.mutable_data_ptr<int>();
+  a.table_stride = B == 1 ? 0 : block_tables.stride(0);
+  a.free_pages = free_pages.const_data_ptr<int>();
+  a.taken = taken.const_data_ptr<int>();
+  a.positions = positions.mutable_data_ptr<int>();
+  a.slots = slots.mutable_data_ptr<int64_t>();
+  a.lengths = lengths.mutable_data_ptr<int>();
+  a.taken_out = taken_out.mutable_data_ptr<int>();
+  a.B = static_cast<int>(B);
+  a.M = static_cast<int>(block_tables.size(1));
+  a.F = static_cast<int>(free_pages.size(0));
+  a.T = static_cast<int>(num_tokens);
+  a.P = static_cast<int>(page_size);
+  nab::assign_pages(at::cuda::getCurrentCUDAStream().stream(), a);
+  return {positions, slots, lengths, taken_out};
+}
+
+void rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+                       const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages, at::Tensor& v_pages,
+                       const OptTensor& q_norm, const OptTensor& k_norm, at::Tensor& out, double eps,
+                       bool interleaved) {
+  constexpr const char* op = "rope_append_paged";
+  const int dtype = half_dtype(op, qkv, "qkv");
+  check_pages(op, k_pages, v_pages, qkv.scalar_type());
+  const int64_t Hkv = k_pages.size(1), P = k_pages.size(2), D = k_pages.size(3);
+  TORCH_CHECK(out.dim() == 3 && out.is_contiguous() && out.size(1) >= 1 && out.size(2) == D &&
+                  out.scalar_type() == qkv.scalar_type() && aligned16(out),
+              op, ": out must be contiguous [tokens, q_heads, ", D, "] of qkv's type");
+  const int64_t T = out.size(0), Hq = out.size(1);
+  TORCH_CHECK(Hq % Hkv == 0, op, ": ", Hq, " query heads do not divide over ", Hkv, " kv heads");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == T && qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1, op,
+              ": qkv must be [", T, ", ", (Hq + 2 * Hkv) * D, "] with contiguous rows");
+  TORCH_CHECK(aligned16(qkv) && qkv.stride(0) % 8 == 0, op, ": the rows of qkv must be 16-byte aligned");
+  TORCH_CHECK(cos.dim() == 2 && cos.is_contiguous() && sin.is_contiguous() && sin.sizes() == cos.sizes() &&
+                  cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.size(0) >= 1,
+              op, ": cos and sin must be contiguous float32 [positions, rotary_dim / 2]");
+  const int64_t R = 2 * cos.size(1);
+  TORCH_CHECK(R % 16 == 0 && R >= 16 && R <= D, op, ": rotary_dim must be a multiple of 16 up to head_dim, got ", R);
+  TORCH_CHECK(cos.size(0) < INT_MAX && aligned16(cos) && aligned16(sin), op, ": cos and sin must be 16-byte aligned");
+  check_vector(op, "positions", positions, at::kInt, T);
+  check_vector(op, "slots", slots, at::kLong, T);
+  for (const auto& [name, w] : {std::pair<const char*, const OptTensor*>{"q_norm", &q_norm}, {"k_norm", &k_norm}}) {
+    if (!*w) continue;
+    check_vector(op, name, **w, qkv.scalar_type(), D);
+    TORCH_CHECK(aligned16(**w), op, ": ", name, " must be 16-byte aligned");
+  }
+  check_devices(op, {{"qkv", &qkv},
+                     {"cos", &cos},
+                     {"sin", &sin},
+                     {"positions", &positions},
+                     {"slots", &slots},
+                     {"k_pages", &k_pages},
+                     {"v_pages", &v_pages},
+                     {"q_norm", q_norm ? &*q_norm : nullptr},
+                     {"k_norm", k_norm ? &*k_norm : nullptr},
+                     {"out", &out}});
+  at::assert_no_overlap(out, qkv);
+  const at::cuda::CUDAGuard guard(qkv.device());
+  nab::RopeAppendArgs a{};
+  a.qkv = qkv.const_data_ptr();
+  a.qkv_stride = qkv.stride(0);
+  a.cos_t = cos.const_data_ptr<float>();
+  a.sin_t = sin.const_data_ptr<float>();
+  a.positions = positions.const_data_ptr<int>();
+  a.slots = slots.const_data_ptr<int64_t>();
+  a.q_norm = q_norm ? q_norm->const_data_ptr() : nullptr;
+  a.k_norm = k_norm ? k_norm->const_data_ptr() : nullptr;
+  a.q_out = out.mutable_data_ptr();
+  a.k_pages = k_pages.mutable_data_ptr();
+  a.v_pages = v_pages.mutable_data_ptr();
+  a.T = T;
+  a.num_slots = k_pages.size(0) * P;
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.D = static_cast<int>(D);
+  a.R = static_cast<int>(R);
+  a.P = static_cast<int>(P);
+  a.max_pos = static_cast<int>(cos.size(0));
+  a.eps = static_cast<float>(eps);
+  nab::rope_append_paged(at::cuda::getCurrentCUDAStream().stream(), a, dtype, interleaved);
+}
+
+void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                     const at::Tensor& block_tables, const at::Tensor& lengths, at::Tensor& out, double scale) {
+  constexpr const char* op = "paged_attention";
+  const int dtype = half_dtype(op, q, "q");
+  check_pages(op, k_pages, v_pages, q.scalar_type());
+  const int64_t Hkv = k_pages.size(1), P = k_pages.size(2), D = k_pages.size(3);
+  TORCH_CHECK(q.dim() == 3 && q.size(1) >= 1 && q.size(2) == D, op, ": q must be [requests, q_heads, ", D, "]");
+  const int64_t B = q.size(0), Hq = q.size(1);
+  TORCH_CHECK(Hq % Hkv == 0, op, ": ", Hq, " query heads do not divide over ", Hkv, " kv heads");
+  TORCH_CHECK(q.stride(2) == 1 && (Hq == 1 || q.stride(1) == D) && aligned16(q) &&
+                  (B <= 1 || (q.stride(0) >= Hq * D && q.stride(0) % D == 0)),
+              op, ": the heads of q must be contiguous and 16-byte aligned, its rows a multiple of head_dim apart");
+  TORCH_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() &&
+                  aligned16(out),
+              op, ": out must be contiguous, of q's shape and type");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == B && block_tables.scalar_type() == at::kInt &&
+                  (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
+              op, ": block_tables must be int32 [", B, ", pages] with contiguous rows");
+  TORCH_CHECK(block_tables.size(1) * P < INT_MAX, op, ": block_tables is too wide");
+  check_vector(op, "lengths", lengths, at::kInt, B);
+  check_devices(op, {{"q", &q},
+                     {"k_pages", &k_pages},
+                     {"v_pages", &v_pages},
+                     {"block_tables", &block_tables},
+                     {"lengths", &lengths},
+                     {"out", &out}});
+  at::assert_no_overlap(out, q);
+  if (B == 0) return;
+  const at::cuda::CUDAGuard guard(q.device());
+  const int sms = sms_of(q);
+  nab::PagedAttnArgs a{};
+  a.q = q.const_data_ptr();
+  a.q_stride = q.stride(0);
+  a.k_pages = k_pages.const_data_ptr();
+  a.v_pages = v_pages.const_data_ptr();
+  a.tables = block_tables.const_data_ptr<int>();
+  a.table_stride = block_tables.stride(0);
+  a.lengths = lengths.const_data_ptr<int>();
+  a.out = out.mutable_data_ptr();
+  a.num_pages = k_pages.size(0);
+  a.B = static_cast<int>(B);
+  a.M = static_cast<int>(block_tables.size(1));
+  a.P = static_cast<int>(P);
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.D = static_cast<int>(D);
+  a.scale = static_cast<float>(scale);
+  // of this call alone: two streams or graphs never share it
+  const at::Tensor ws = at::empty({nab::paged_attention_ws_floats(a.B, a.M, a.P, a.Hq, a.Hkv, a.D, sms)},
+                                  q.options().dtype(at::kFloat));
+  a.ws = ws.mutable_data_ptr<float>();
+  nab::paged_attention(at::cuda::getCurrentCUDAStream().stream(), a, dtype, sms);
+}
+
+using LogprobsResult = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+LogprobsResult token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t top_k,
+                              int64_t vocab_start) {
+  constexpr const char* op = "token_logprobs";
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1), op,
+              ": logits must be [rows, vocabulary] with contiguous rows");
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V < (1 << 30), op, ": the vocabulary is too large");
+  int dtype = nab::kF32;
+  if (logits.scalar_type() != at::kFloat) {
+    TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf, op,
+                ": logits must be float32, float16 or bfloat16, got ", logits.scalar_type());
+    dtype = logits.scalar_type() == at::kHalf ? nab::kF16 : nab::kBF16;
+  }
+  check_vector(op, "tokens", tokens, at::kLong, rows);
+  TORCH_CHECK(top_k >= 0 && top_k <= nab::kMaxTopK && top_k <= V, op, ": top_k must be from 0 to ", nab::kMaxTopK,
+              " and at most the vocabulary, got ", top_k);
+  TORCH_CHECK(vocab_start >= 0, op, ": vocab_start must not be negative");
+  check_devices(op, {{"logits", &logits}, {"tokens", &tokens}});
+  const at::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor logprob = at::empty({rows}, f32), entropy = at::empty({rows}, f32), lse = at::empty({rows}, f32);
+  at::Tensor top_logprobs = at::empty({rows, top_k}, f32), top_tokens = at::empty({rows, top_k}, tokens.options());
+  at::Tensor top_logits = at::empty({rows, top_k}, f32);
+  nab::LogprobsArgs a{};
+  a.logits = logits.const_data_ptr();
+  a.stride = logits.stride(0);
+  a.tokens = tokens.const_data_ptr<int64_t>();
+  a.vocab_start = vocab_start;
+  a.logprob = logprob.mutable_data_ptr<float>();
+  a.entropy = entropy.mutable_data_ptr<float>();
+  a.lse = lse.mutable_data_ptr<float>();
+  a.top_logprobs = top_logprobs.mutable_data_ptr<float>();
+  a.top_tokens = top_tokens.mutable_data_ptr<int64_t>();
+  a.top_logits = top_logits.mutable_data_ptr<float>();
+  a.rows = rows;
+  a.V = static_cast<int>(V);
+  a.top_k = static_cast<int>(top_k);
+  nab::token_logprobs(at::cuda::getCurrentCUDAStream().stream(), a, dtype, sms_of(logits));
+  return {logprob, entropy, lse, top_logprobs, top_tokens, top_logits};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(nab, m) {
+  constexpr auto any = c10::DispatchKey::CompositeExplicitAutograd;
+  m.def("assign_pages(Tensor cached, Tensor? query_start, Tensor(a!) block_tables, Tensor free_pages, Tensor taken, "
+        "int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.impl("assign_pages", torch::dispatch(any, TORCH_FN(assign_pages)));
+  m.def("rope_append_paged(Tensor qkv, Tensor cos, Tensor sin, Tensor positions, Tensor slots, Tensor(a!) k_pages, "
+        "Tensor(b!) v_pages, Tensor? q_norm, Tensor? k_norm, Tensor(c!) out, float eps, bool interleaved) -> ()");
+  m.impl("rope_append_paged", torch::dispatch(any, TORCH_FN(rope_append_paged)));
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, "
+        "Tensor(a!) out, float scale) -> ()");
+  m.impl("paged_attention", torch::dispatch(any, TORCH_FN(paged_attention)));
+  m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k, int vocab_start) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.impl("token_logprobs", torch::dispatch(any, TORCH_FN(token_logprobs)));
+}

@@ -39,12 +39,15 @@ CORE_SOURCES = [
     "nab_gemm_sm100.cu",
     "nab_llama.cu",
     "nab_attn_sm100.cu",
+    "nab_paged.cu",
+    "nab_paged_attn.cu",
+    "nab_logprobs.cu",
     "nab_comm.cpp",
     "nab_kerr.cpp",
     "nab_nvls.cpp",
     "nab_capi.cpp",
 ]
-TORCH_SOURCES = ["nab_torch.cpp"]
+TORCH_SOURCES = ["nab_torch.cpp", "nab_torch_serve.cpp"]
 # Linked into libnab.so only: the allocation-free entry point, whose static
 # scratch array should not ride along in the torch extension.
 PLAIN_ONLY_SOURCES = ["nab_noalloc.cu"]

@@ -1,0 +1,65 @@
+"""Log-probabilities of given tokens, with entropy and top alternatives."""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Sequence
+
+import torch
+
+from . import _ext
+from .errors import after_launch
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` gives for each row of logits (fp32, token ids int64)."""
+
+    logprob: torch.Tensor       # [rows]: of the given token, -inf if it is not in this part of the vocabulary
+    entropy: torch.Tensor       # [rows]: of the distribution, in nats
+    lse: torch.Tensor           # [rows]: log of the sum of exp(logits)
+    top_logprobs: torch.Tensor  # [rows, top_k], falling
+    top_tokens: torch.Tensor    # [rows, top_k]
+    top_logits: torch.Tensor    # [rows, top_k]: the logits themselves, by which shards are merged
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, vocab_start: int = 0) -> TokenLogprobs:
+    """Log-softmax of ``logits[rows, vocabulary]`` at ``tokens``, and its entropy and ``top_k`` largest entries.
+
+    One launch that reads the logits (fp32, fp16 or bf16; rows may be further
+    apart than the vocabulary) once; sums in fp32. ``top_k`` is at most 32;
+    equal logits rank by the lowest token id. Entries of -inf (masked tokens)
+    have probability 0. A row that holds NaN or +inf, or only -inf, gives NaN
+    (``lse`` of the last is -inf); NaN ranks as -inf.
+
+    ``logits`` may be one shard of the vocabulary, with column 0 the token
+    ``vocab_start``: the result is that of the shard alone, and
+    :func:`join_token_logprobs` makes the whole vocabulary's from all shards.
+    For inference: logits that require a gradient are refused.
+    """
+    ops = _ext.load()
+    r = TokenLogprobs(*ops.token_logprobs(logits, tokens, top_k, vocab_start))
+    after_launch()
+    return r
+
+
+def join_token_logprobs(shards: Sequence[TokenLogprobs]) -> TokenLogprobs:
+    """The results of every vocabulary shard (in order of the shards, for the
+    same tokens and top_k) as those of the whole vocabulary."""
+    if not shards:
+        raise ValueError("join_token_logprobs needs at least one shard")
+    part = torch.stack([s.lse for s in shards])  # [shards, rows]
+    lse = part.logsumexp(0)
+    shift = part - lse  # log of a shard's probability
+    weight = shift.exp()
+    # a shard whose tokens are all masked has no distribution of its own (NaN): it adds nothing
+    masked = (part == -torch.inf) & (lse != -torch.inf)
+    entropy = torch.where(masked, 0, weight * (torch.stack([s.entropy for s in shards]) - shift)).sum(0)
+    logprob = torch.where(masked, -torch.inf, torch.stack([s.logprob for s in shards]) + shift).amax(0)
+    top = torch.cat([torch.where(m[:, None], -torch.inf, s.top_logprobs + d[:, None])
+                     for s, d, m in zip(shards, shift, masked)], -1)
+    ids = torch.cat([s.top_tokens for s in shards], -1)
+    raw = torch.cat([s.top_logits for s in shards], -1)
+    k = shards[0].top_logprobs.shape[1]
+    # by the logits, which are exact (NaN as -inf); stable: equal ones keep the order of the token ids
+    order = raw.nan_to_num(nan=-torch.inf, posinf=torch.inf, neginf=-torch.inf)
+    order = order.argsort(dim=-1, descending=True, stable=True)[:, :k]
+    return TokenLogprobs(logprob, entropy, lse, top.gather(-1, order), ids.gather(-1, order), raw.gather(-1, order))
