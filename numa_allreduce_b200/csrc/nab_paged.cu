@@ -137,28 +137,32 @@ struct RopeAppendDev {
 // one rounding at the end. k and v go to their page row, q to q_out.
 //
 // Bound by memory: each value is read and written once. One group of D / 16
-// lanes per (token, kHeads consecutive heads); a lane holds two 16-byte
-// pieces of each head so that a rotary pair lies in one lane: half layout,
-// dims [8c, 8c + 8) and [R/2 + 8c, ...); interleaved, dims [16c, 16c + 16);
-// the lanes past R / 16 hold the rest of the head unrotated. The token's
-// cos and sin stay in registers over the heads.
+// lanes per token and run of kHeads heads; a lane holds two 16-byte pieces
+// of each head so that a rotary pair lies in one lane: half layout, dims
+// [8c, 8c + 8) and [R/2 + 8c, ...); interleaved, dims [16c, 16c + 16); the
+// lanes past R / 16 hold the rest of the head unrotated. The loads of all
+// heads of a run are in flight together, and the token's cos and sin and the
+// norm's weight stay in registers over them. A run is of q heads, of k heads
+// or of v heads, the same for a whole block, and consecutive blocks take the
+// runs of the same tokens (their cos and sin rows and cache lines of qkv).
 template <typename T, int D, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(256) k_rope_append_paged(const __grid_constant__ RopeAppendDev p) {
-  constexpr int kLanes = D / 16;
+  constexpr int kLanes = D / 16, kTokens = 256 / kLanes;
   const RopeAppendArgs& a = p.a;
   pdl_wait();
   pdl_trigger();
-  const int H = a.Hq + 2 * a.Hkv;
-  const int chunks = (H + kHeads - 1) / kHeads;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const bool live = item < a.T * chunks;
-  // lanes past the end follow the last item without storing: the shuffles need the whole warp
-  const int64_t at = live ? item : a.T * chunks - 1;
-  const int64_t t = at / chunks;
-  const int h0 = static_cast<int>(at % chunks) * kHeads;
+  const int q_runs = (a.Hq + kHeads - 1) / kHeads, kv_runs = (a.Hkv + kHeads - 1) / kHeads;
+  const unsigned runs = q_runs + 2 * kv_runs;
+  const int run = static_cast<int>(blockIdx.x % runs);
+  const int64_t token = static_cast<int64_t>(blockIdx.x / runs) * kTokens + threadIdx.x / kLanes;
+  const bool live = token < a.T;
+  // lanes past the end follow the last token without storing: the shuffles need the whole warp
+  const int64_t t = live ? token : a.T - 1;
+  const bool is_q = run < q_runs, is_v = run >= q_runs + kv_runs;
+  const int h0 = (is_q ? run : is_v ? run - q_runs - kv_runs : run - q_runs) * kHeads;  // within its kind
+  const int heads = min(kHeads, (is_q ? a.Hq : a.Hkv) - h0);
   const int c = threadIdx.x % kLanes;
-  const int nrot = a.R / 16;
-  const bool rotated = c < nrot;
+  const bool rotated = c < a.R / 16;
   int d0, d1;  // the lane's two pieces of 8 dims
   if (kInterleaved || !rotated) {
     d0 = 16 * c;
@@ -167,22 +171,52 @@ __global__ void __launch_bounds__(256) k_rope_append_paged(const __grid_constant
     d0 = 8 * c;
     d1 = a.R / 2 + 8 * c;
   }
-  int pos = a.positions[t];
-  int64_t slot = a.slots[t];
-  if (pos < 0 || pos >= a.max_pos || slot >= a.num_slots) {
-    if (live && c == 0 && h0 == 0)
-      record_local_failure(p.err, p.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(t));
-    pos = min(max(pos, 0), a.max_pos - 1);
-    if (slot >= a.num_slots) slot = -1;
+  const T* src = static_cast<const T*>(a.qkv) + t * a.qkv_stride +
+                 static_cast<int64_t>((is_q ? 0 : is_v ? a.Hq + a.Hkv : a.Hq) + h0) * D;
+  uint4 raw[kHeads][2];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = kHeads == 1 ? 0 : min(i, heads - 1);
+    raw[i][0] = ld_plain(src + h * D + d0);
+    raw[i][1] = ld_plain(src + h * D + d1);
   }
-  const int64_t page = slot / a.P;
-  const int row = static_cast<int>(slot - page * a.P);
-  const T* src = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
+
+  // where the run's first head goes, and the distance between heads
+  T* dst;
+  int64_t step = D;
+  bool store = live;
+  if (is_q) {
+    dst = static_cast<T*>(a.q_out) + (t * a.Hq + h0) * D;
+  } else {
+    const int64_t slot = a.slots[t];
+    store = live && slot >= 0 && slot < a.num_slots;
+    if (live && slot >= a.num_slots && h0 == 0 && !is_v && c == 0)
+      record_local_failure(p.err, p.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(t));
+    const uint32_t at = store ? static_cast<uint32_t>(slot) : 0u;  // below num_slots, which fits 32 bits
+    const uint32_t page = at / static_cast<uint32_t>(a.P), row = at - page * a.P;
+    dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) + ((static_cast<int64_t>(page) * a.Hkv + h0) * a.P + row) * D;
+    step = static_cast<int64_t>(a.P) * D;
+  }
+  if (is_v) {
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (!store || i >= heads) break;
+      st_plain(dst + i * step + d0, raw[i][0]);
+      st_plain(dst + i * step + d1, raw[i][1]);
+    }
+    return;
+  }
 
   // half layout: angle e belongs to dims (d0 + e, d1 + e); interleaved: to
   // (16c + 2e, 16c + 2e + 1)
   float cs[8], sn[8];
-  if (rotated && h0 < a.Hq + a.Hkv) {
+  if (rotated) {
+    int pos = a.positions[t];
+    if (pos < 0 || pos >= a.max_pos) {
+      if (live && is_q && h0 == 0 && c == 0)
+        record_local_failure(p.err, p.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(t));
+      pos = min(max(pos, 0), a.max_pos - 1);
+    }
     const float4* ct = reinterpret_cast<const float4*>(a.cos_t + static_cast<int64_t>(pos) * (a.R / 2) + 8 * c);
     const float4* st = reinterpret_cast<const float4*>(a.sin_t + static_cast<int64_t>(pos) * (a.R / 2) + 8 * c);
 #pragma unroll
@@ -192,74 +226,56 @@ __global__ void __launch_bounds__(256) k_rope_append_paged(const __grid_constant
       sn[4 * k] = y.x, sn[4 * k + 1] = y.y, sn[4 * k + 2] = y.z, sn[4 * k + 3] = y.w;
     }
   }
-  uint4 raw[kHeads][2];
-#pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = min(h0 + i, H - 1);
-    raw[i][0] = ld_plain(src + static_cast<int64_t>(h) * D + d0);
-    raw[i][1] = ld_plain(src + static_cast<int64_t>(h) * D + d1);
+  const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
+  uint4 wr[2] = {};
+  if (w != nullptr) {
+    wr[0] = __ldg(reinterpret_cast<const uint4*>(w + d0));
+    wr[1] = __ldg(reinterpret_cast<const uint4*>(w + d1));
   }
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-    uint4 out0 = raw[i][0], out1 = raw[i][1];
     Acc<T> x0, x1;
-    acc_set(x0, out0);
-    acc_set(x1, out1);
-    const T* w = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
-    if (a.q_norm != nullptr || a.k_norm != nullptr) {  // the same for every lane
+    acc_set(x0, raw[i][0]);
+    acc_set(x1, raw[i][1]);
+    if (w != nullptr) {  // the same for the whole block
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x0.v[e] * x0.v[e] + x1.v[e] * x1.v[e];
 #pragma unroll
       for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (w != nullptr && !is_v) {
-        const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-        Acc<T> w0, w1;
-        acc_set(w0, __ldg(reinterpret_cast<const uint4*>(w + d0)));
-        acc_set(w1, __ldg(reinterpret_cast<const uint4*>(w + d1)));
+      const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+      Acc<T> w0, w1;
+      acc_set(w0, wr[0]);
+      acc_set(w1, wr[1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x0.v[e] *= inv * w0.v[e];
+        x1.v[e] *= inv * w1.v[e];
+      }
+    }
+    if (rotated) {
+      if (kInterleaved) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u0 = x0.v[2 * e], v0 = x0.v[2 * e + 1], u1 = x1.v[2 * e], v1 = x1.v[2 * e + 1];
+          x0.v[2 * e] = u0 * cs[e] - v0 * sn[e];
+          x0.v[2 * e + 1] = v0 * cs[e] + u0 * sn[e];
+          x1.v[2 * e] = u1 * cs[4 + e] - v1 * sn[4 + e];
+          x1.v[2 * e + 1] = v1 * cs[4 + e] + u1 * sn[4 + e];
+        }
+      } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x0.v[e] *= inv * w0.v[e];
-          x1.v[e] *= inv * w1.v[e];
+          const float u = x0.v[e], v = x1.v[e];
+          x0.v[e] = u * cs[e] - v * sn[e];
+          x1.v[e] = v * cs[e] + u * sn[e];
         }
       }
     }
-    if (!is_v) {
-      if (rotated) {
-        if (kInterleaved) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u0 = x0.v[2 * e], v0 = x0.v[2 * e + 1], u1 = x1.v[2 * e], v1 = x1.v[2 * e + 1];
-            x0.v[2 * e] = u0 * cs[e] - v0 * sn[e];
-            x0.v[2 * e + 1] = v0 * cs[e] + u0 * sn[e];
-            x1.v[2 * e] = u1 * cs[4 + e] - v1 * sn[4 + e];
-            x1.v[2 * e + 1] = v1 * cs[4 + e] + u1 * sn[4 + e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float u = x0.v[e], v = x1.v[e];
-            x0.v[e] = u * cs[e] - v * sn[e];
-            x1.v[e] = v * cs[e] + u * sn[e];
-          }
-        }
-      }
-      out0 = acc_pack(x0);
-      out1 = acc_pack(x1);
+    if (store && i < heads) {
+      st_plain(dst + i * step + d0, acc_pack(x0));
+      st_plain(dst + i * step + d1, acc_pack(x1));
     }
-    if (!live || h >= H) continue;
-    T* dst;
-    if (is_q) {
-      dst = static_cast<T*>(a.q_out) + (t * a.Hq + h) * D;
-    } else {
-      if (slot < 0) continue;
-      const int kvh = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
-      dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) + ((page * a.Hkv + kvh) * a.P + row) * D;
-    }
-    st_plain(dst + d0, out0);
-    st_plain(dst + d1, out1);
   }
 }
 
@@ -281,11 +297,23 @@ void launch(void (*kernel)(KArgs...), int64_t grid, int block, size_t smem, cuda
   if (e != cudaSuccess) throw std::runtime_error(std::string(what) + " launch failed: " + cudaGetErrorString(e));
 }
 
+template <typename T, int D, bool kInterleaved, int kHeads>
+void launch_runs(cudaStream_t s, const RopeAppendDev& p) {
+  constexpr int kTokens = 256 / (D / 16);
+  const int64_t runs = (p.a.Hq + kHeads - 1) / kHeads + 2 * ((p.a.Hkv + kHeads - 1) / kHeads);
+  launch(k_rope_append_paged<T, D, kInterleaved, kHeads>, (p.a.T + kTokens - 1) / kTokens * runs, 256, 0, s,
+         "rope_append_paged", p);
+}
+
 template <typename T, int D, bool kInterleaved>
 void launch_append(cudaStream_t s, const RopeAppendDev& p) {
-  const int H = p.a.Hq + 2 * p.a.Hkv;
-  launch(k_rope_append_paged<T, D, kInterleaved, 1>, (p.a.T * H * (D / 16) + 255) / 256, 256, 0, s, "rope_append_paged",
-         p);
+  // one head per group while that fills the GPU's threads less than twice, else runs of 4
+  const int64_t threads = p.a.T * (p.a.Hq + 2 * p.a.Hkv) * (D / 16);
+  if (threads <= 2 * 148 * 2048) {
+    launch_runs<T, D, kInterleaved, 1>(s, p);
+  } else {
+    launch_runs<T, D, kInterleaved, 4>(s, p);
+  }
 }
 
 template <typename T>
