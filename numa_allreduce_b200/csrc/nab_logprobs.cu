@@ -70,28 +70,101 @@ NAB_DINLINE uint64_t key_of(float x, uint32_t index) {
   return (static_cast<uint64_t>(ordered(x)) << 32) | (0xffffffffu - index);
 }
 
-// Running statistics: m >= every value so far (at least -FLT_MAX), S = sum
-// exp(x - m), U = sum log2(e) (x - m) exp(x - m).
+// Two floats in one 64-bit register: sm_100 adds and multiplies them in one instruction.
+NAB_DINLINE uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+NAB_DINLINE float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+NAB_DINLINE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+NAB_DINLINE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+NAB_DINLINE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// How a piece of 16 bytes is read: its kN elements as pairs of floats, its
+// largest element (NaN left out), a word of -inf, and how many of the lowest
+// bits of `ordered` are the same for every value of the type and sign.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<float> {
+  static constexpr uint32_t kFill = 0xff800000u;
+  static constexpr int kDrop = 0;
+  NAB_DINLINE static float largest(uint4 w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  NAB_DINLINE static void pairs(uint4 w, uint64_t (&v)[2]) {
+    v[0] = pair(__uint_as_float(w.x), __uint_as_float(w.y));
+    v[1] = pair(__uint_as_float(w.z), __uint_as_float(w.w));
+  }
+};
+template <>
+struct Piece<__nv_bfloat16> {
+  static constexpr uint32_t kFill = 0xff80ff80u;
+  static constexpr int kDrop = 16;
+  NAB_DINLINE static float largest(uint4 w) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+    return fmaxf(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  NAB_DINLINE static void pairs(uint4 w, uint64_t (&v)[4]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pair(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+  }
+};
+template <>
+struct Piece<__half> {
+  static constexpr uint32_t kFill = 0xfc00fc00u;
+  static constexpr int kDrop = 13;
+  NAB_DINLINE static float largest(uint4 w) {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+    const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(m.x, m.y);
+  }
+  NAB_DINLINE static void pairs(uint4 w, uint64_t (&v)[4]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[i] = pair(f.x, f.y);
+    }
+  }
+};
+
+// S = sum exp(x - m) and U = sum log2(e) (x - m) exp(x - m) for m >= every x
+// so far (m >= -FLT_MAX).
 struct Stats {
   float m, s, u;
 };
+// exponents below -1000 count as -1000 (exp2 of them is zero), which keeps 0 * inf out
+NAB_DINLINE float exponent(float from, float to) { return fmaxf((from - to) * kL2e, -1000.f); }
 NAB_DINLINE void raise(Stats& a, float m) {
-  // exponents below -1000 count as zero (exp2 of them is), which keeps 0 * inf out
-  const float d = fmaxf((a.m - m) * kL2e, -1000.f);
-  const float f = lp_ex2(d);
+  const float d = exponent(a.m, m), f = lp_ex2(d);
   a.u = f * (a.u + d * a.s);
   a.s *= f;
   a.m = m;
 }
-NAB_DINLINE Stats merge(Stats a, Stats b) {
-  const float m = fmaxf(a.m, b.m);
-  raise(a, m);
-  raise(b, m);
-  return {m, a.s + b.s, a.u + b.u};
-}
 
 struct LpShared {
-  Stats warp_stats[kLpWarps];
+  float warp_m[kLpWarps], warp_s[kLpWarps], warp_u[kLpWarps];
   Stats stats;                    // this CTA's, read by the cluster's first CTA
   uint64_t top[kMaxTopK];         // this CTA's largest keys, in order; 0 past its elements
   uint64_t cand[kCand];
@@ -100,46 +173,40 @@ struct LpShared {
   int n_who, n_cand;
 };
 
-// The largest t with at least k threads' keys >= t (0 if fewer than k keys
-// are above 0): bisection from the top bit, which ends once exactly k are left.
-NAB_DINLINE uint64_t kth_largest(uint64_t key, int k) {
+// A cut with at least k threads' keys at or above it (0 if fewer than k keys
+// are above 0), found bit by bit from `bits` down. Any such cut is right; it
+// ends once no more than `slack` threads too many are left.
+NAB_DINLINE uint64_t cut_of(uint64_t key, int k, int bits, int slack) {
   if (__syncthreads_count(key != 0) < k) return 0;
   uint64_t t = 0;
-  for (int bit = 63; bit >= 0; --bit) {
+  for (int bit = bits - 1; bit >= 0; --bit) {
     const uint64_t c = t | (uint64_t{1} << bit);
     const int n = __syncthreads_count(key >= c);
     if (n >= k) t = c;
-    if (n == k) break;
+    if (n >= k && n <= k + slack) break;
   }
   return t;
 }
 
+// A row as pieces of 16 aligned bytes: piece p holds the elements
+// [p * kN - mis, (p + 1) * kN - mis), of which the first and the last piece
+// may have some outside [0, V).
 template <typename T>
 struct Row {
-  static constexpr int kN = VecT<T>::kN;  // elements of a piece
-  const T* x;       // the row
-  int mis;          // elements between the 16-byte boundary before x and x
+  static constexpr int kN = VecT<T>::kN;
+  const T* x;
+  int mis;  // elements between the 16-byte boundary before x and x
   int V;
-  // piece p holds the elements [p * kN - mis, ...); those outside [0, V) read as `fill`
-  NAB_DINLINE bool inner(int p) const { return p * kN >= mis && (p + 1) * kN - mis <= V; }
-  NAB_DINLINE void load(int p, Acc<T>& a, float fill) const {
-    const T* at = x + (static_cast<int64_t>(p) * kN - mis);
-    if (inner(p)) {
-      acc_set(a, ld_plain(at));
-    } else {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const int i = p * kN - mis + e;
-        a.v[e] = i >= 0 && i < V ? static_cast<float>(at[e]) : fill;
-      }
-    }
-  }
+  NAB_DINLINE int first(int p) const { return p * kN - mis; }
+  NAB_DINLINE bool inner(int p) const { return first(p) >= 0 && first(p) + kN <= V; }
+  NAB_DINLINE uint4 whole(int p) const { return ld_plain(x + first(p)); }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster) {
   __shared__ LpShared sh;
   constexpr int N = Row<T>::kN;
+  constexpr int kBatch = 4;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -151,90 +218,136 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   r.V = a.V;
   const int pieces = (r.mis + a.V + N - 1) / N;
   const int per = (pieces + cluster - 1) / cluster;
-  const int p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);
+  const int p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);  // this CTA's pieces
+  const int i0 = max(p0, r.mis > 0), i1 = min(p1, (r.mis + a.V) / N);  // those within the row
   const int k = a.top_k;
+  float picked = -INFINITY;  // the given token's logit
+  if (tid == 0 && part == 0) {
+    const int64_t at = a.tokens[row] - a.vocab_start;
+    if (at >= 0 && at < a.V) picked = static_cast<float>(r.x[at]);
+  }
 
   // ------------------------------------------------------- one pass --
-  Stats st = {-FLT_MAX, 0.f, 0.f};
-  float kv = -INFINITY;  // largest value so far, first held by piece kp
+  // Piece p is thread (p - p0) % kLpThreads's. Batches of kBatch pieces, the
+  // next one's loads in flight during one's arithmetic; pieces past the end
+  // read as -inf, which adds exactly nothing.
+  float m = -FLT_MAX, kv = -INFINITY;  // kv: the largest value so far, first held by piece kp
   int kp = p0 + tid;
-  auto take = [&](const Acc<T>& v, int p, int n_valid_mask) {
-    float mx = v.v[0];
+  uint64_t s2 = 0, u2 = 0;
+  const uint64_t l2e = pair(kL2e, kL2e);
+  auto fetch = [&](int p, uint4 (&w)[kBatch]) {
 #pragma unroll
-    for (int e = 1; e < N; ++e) mx = fmaxf(mx, v.v[e]);
-    if (mx > kv) {
-      kv = mx;
-      kp = p;
-      if (mx > st.m) raise(st, mx);
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float d = max_nan((v.v[e] - st.m) * kL2e, -1000.f);
-      const float w = lp_ex2(d);
-      if ((n_valid_mask >> e) & 1) {
-        st.s += w;
-        st.u += d * w;
-      }
+    for (int b = 0; b < kBatch; ++b) {
+      w[b] = make_uint4(Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill);
+      if (p + b * kLpThreads < i1) w[b] = r.whole(p + b * kLpThreads);
     }
   };
-  constexpr int kUnroll = 4;
   int p = p0 + tid;
-  for (; p + (kUnroll - 1) * kLpThreads < p1; p += kUnroll * kLpThreads) {
-    if (r.inner(p) && r.inner(p + (kUnroll - 1) * kLpThreads)) {
-      Acc<T> v[kUnroll];
-      uint4 raw[kUnroll];
+  if (p < i0) p += kLpThreads;
+  uint4 cur[kBatch];
+  fetch(p, cur);
+  while (p < i1) {
+    uint4 next[kBatch];
+    fetch(p + kBatch * kLpThreads, next);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) raw[u] = ld_plain(r.x + (static_cast<int64_t>(p + u * kLpThreads) * N - r.mis));
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        acc_set(v[u], raw[u]);
-        take(v[u], p + u * kLpThreads, (1 << N) - 1);
-      }
-    } else {
-      for (int u = 0; u < kUnroll; ++u) {
-        const int q = p + u * kLpThreads;
-        Acc<T> v;
-        r.load(q, v, -INFINITY);
-        int mask = 0;
-        for (int e = 0; e < N; ++e) mask |= (q * N - r.mis + e >= 0 && q * N - r.mis + e < a.V) << e;
-        take(v, q, mask);
+    for (int b = 0; b < kBatch; ++b) {
+      const float mx = Piece<T>::largest(cur[b]);
+      if (mx > kv) {
+        kv = mx;
+        kp = p + b * kLpThreads;
       }
     }
-  }
-  for (; p < p1; p += kLpThreads) {
-    Acc<T> v;
-    r.load(p, v, -INFINITY);
-    int mask = (1 << N) - 1;
-    if (!r.inner(p)) {
-      mask = 0;
-      for (int e = 0; e < N; ++e) mask |= (p * N - r.mis + e >= 0 && p * N - r.mis + e < a.V) << e;
+    {
+      const float to = fmaxf(m, kv);
+      const float d = exponent(m, to), f = lp_ex2(d);
+      const uint64_t f2 = pair(f, f);
+      u2 = mul2(f2, fma2(pair(d, d), s2, u2));
+      s2 = mul2(f2, s2);
+      m = to;
     }
-    take(v, p, mask);
+    const uint64_t neg = pair(-m, -m);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      uint64_t v[N / 2];
+      Piece<T>::pairs(cur[b], v);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const float2 d = unpair(mul2(add2(v[e], neg), l2e));
+        const float d0 = max_nan(d.x, -1000.f), d1 = max_nan(d.y, -1000.f);
+        const uint64_t w = pair(lp_ex2(d0), lp_ex2(d1));
+        s2 = add2(s2, w);
+        u2 = fma2(pair(d0, d1), w, u2);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) cur[b] = next[b];
+    p += kBatch * kLpThreads;
   }
+  const float2 s_ = unpair(s2), u_ = unpair(u2);
+  Stats st = {m, s_.x + s_.y, u_.x + u_.y};
+  // the row's first and last piece, where they reach past it
+  auto edge = [&](int q) {
+    if (q < p0 || q >= p1 || r.inner(q) || (q - p0) % kLpThreads != tid) return;
+    for (int e = 0; e < N; ++e) {
+      const int i = r.first(q) + e;
+      if (i < 0 || i >= a.V) continue;
+      const float x = static_cast<float>(r.x[i]);
+      if (x > kv || (x == kv && q < kp)) {
+        kv = x;
+        kp = q;
+      }
+      if (x > st.m) raise(st, x);
+      const float d = max_nan((x - st.m) * kL2e, -1000.f), w = lp_ex2(d);
+      st.s += w;
+      st.u += d * w;
+    }
+  };
+  edge(0);
+  if (pieces > 1) edge(pieces - 1);
 
   // ------------------------------------------------ statistics of the CTA --
-  Stats all = st;
+  float top = st.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Stats b = {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
-                     __shfl_xor_sync(0xffffffffu, all.u, o)};
-    all = merge(all, b);
-  }
-  if (lane == 0) sh.warp_stats[warp] = all;
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) sh.warp_m[warp] = top;
   if (tid < kMaxTopK) sh.top[tid] = 0;
   if (tid == 0) sh.n_who = sh.n_cand = 0;
   __syncthreads();
-  if (tid == 0) {
-    Stats b = sh.warp_stats[0];
-    for (int w = 1; w < kLpWarps; ++w) b = merge(b, sh.warp_stats[w]);
-    sh.stats = b;
+  top = sh.warp_m[lane % kLpWarps];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  raise(st, top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+    st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
+  }
+  if (lane == 0) {
+    sh.warp_s[warp] = st.s;
+    sh.warp_u[warp] = st.u;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    float s = lane < kLpWarps ? sh.warp_s[lane] : 0.f, u = lane < kLpWarps ? sh.warp_u[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    if (lane == 0) sh.stats = {top, s, u};
   }
 
   // ------------------------------------------------------ top k of the CTA --
   if (k > 0) {
+    // (value, piece within the CTA), larger = earlier, in as few bits as it takes
+    const int piece_bits = 32 - __clz(p1 - p0);
+    auto piece_key = [&](float x, int q) {
+      return (static_cast<uint64_t>(ordered(x) >> Piece<T>::kDrop) << piece_bits) |
+             static_cast<uint64_t>(p1 - 1 - q);
+    };
     const bool has = p0 + tid < p1;
-    const uint64_t key = has ? key_of(kv, static_cast<uint32_t>(kp)) : 0;
-    const uint64_t cut = kth_largest(key, k);
+    const uint64_t key = has ? piece_key(kv, kp) : 0;
+    const uint64_t cut = cut_of(key, k, 32 - Piece<T>::kDrop + piece_bits, 12);
     if (has && key >= cut) sh.who[atomicAdd(&sh.n_who, 1)] = tid;
     __syncthreads();
     const int n_who = sh.n_who;
@@ -243,14 +356,17 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       for (int i = tid; i < n_who * depth; i += kLpThreads) {
         const int q = p0 + sh.who[i / depth] + (i % depth) * kLpThreads;
         if (q >= p1) continue;
-        Acc<T> v;
-        r.load(q, v, -INFINITY);
+        if (r.inner(q)) {
+          Acc<T> v;
+          acc_set(v, r.whole(q));
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int index = q * N - r.mis + e;
-          // as a thread's key would rank it, so that equal values of later pieces stay out
-          if (index >= 0 && index < a.V && key_of(v.v[e], static_cast<uint32_t>(q)) >= cut)
-            f(key_of(v.v[e], static_cast<uint32_t>(index)));
+          for (int e = 0; e < N; ++e)
+            if (piece_key(v.v[e], q) >= cut) f(key_of(v.v[e], static_cast<uint32_t>(r.first(q) + e)));
+        } else {
+          for (int j = max(0, r.first(q)); j < min(a.V, r.first(q) + N); ++j) {
+            const float x = static_cast<float>(r.x[j]);
+            if (piece_key(x, q) >= cut) f(key_of(x, static_cast<uint32_t>(j)));
+          }
         }
       }
     };
@@ -292,13 +408,16 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   // ---------------------------------------------------- join of the cluster --
   if (cluster > 1) sm100::cluster_sync(); else __syncthreads();
   if (part == 0) {
-    Stats b = sh.stats;
+    Stats all = sh.stats;
     uint64_t mine = 0;
     if (cluster > 1) {
-      const uint32_t stats_at = sm100::smem_u32(&sh.stats);
-      for (int c = 1; c < cluster; ++c) {
-        const uint32_t at = sm100::dsmem_addr(stats_at, c);
-        b = merge(b, {sm100::ld_dsmem_f32(at), sm100::ld_dsmem_f32(at + 4), sm100::ld_dsmem_f32(at + 8)});
+      // every thread adds the CTAs up for itself, in their order
+      Stats part_[kMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {
+        const uint32_t at = sm100::dsmem_addr(sm100::smem_u32(&sh.stats), c < cluster ? c : 0);
+        part_[c] = {sm100::ld_dsmem_f32(at), sm100::ld_dsmem_f32(at + 4), sm100::ld_dsmem_f32(at + 8)};
+        all.m = fmaxf(all.m, part_[c].m);
       }
       // keys of every CTA, one per thread (8 x 32 at most); all are different
       if (tid < cluster * k) {
@@ -307,18 +426,24 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
         mine = (static_cast<uint64_t>(hi) << 32) | lo;
       }
       if (tid < kMaxCluster * kMaxTopK) sh.cand[tid] = mine;
+      all.s = all.u = 0.f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {
+        raise(part_[c], all.m);
+        all.s += c < cluster ? part_[c].s : 0.f;
+        all.u += c < cluster ? part_[c].u : 0.f;
+      }
       __syncthreads();
     } else if (tid < k) {
       mine = sh.top[tid];
     }
-    const float log2_s = log2f(b.s);
+    const float log2_s = log2f(all.s);
     if (tid == 0) {
       const int64_t at = a.tokens[row] - a.vocab_start;
-      float lp = -INFINITY;
-      if (at >= 0 && at < a.V) lp = (static_cast<float>(r.x[at]) - b.m) - log2_s * kLn2;
-      a.logprob[row] = lp;
-      a.lse[row] = b.m + log2_s * kLn2;
-      a.entropy[row] = (log2_s - b.u / b.s) * kLn2;
+      const bool here = at >= 0 && at < a.V;
+      a.logprob[row] = here ? (picked - all.m) - log2_s * kLn2 : -INFINITY;
+      a.lse[row] = all.m + log2_s * kLn2;
+      a.entropy[row] = (log2_s - all.u / all.s) * kLn2;
     }
     if (mine != 0) {
       int rank = tid;
@@ -328,7 +453,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       }
       if (rank < k) {
         const float x = unordered(static_cast<uint32_t>(mine >> 32));
-        a.top_logprobs[row * k + rank] = (x - b.m) - log2_s * kLn2;
+        a.top_logprobs[row * k + rank] = (x - all.m) - log2_s * kLn2;
         a.top_logits[row * k + rank] = x;
         a.top_tokens[row * k + rank] = static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(mine)) + a.vocab_start;
       }
