@@ -37,6 +37,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <stdexcept>
 #include <string>
@@ -708,8 +709,14 @@ void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
   a.timeout_ns = kernel_timeout_ns();
   const void* kernel = p.GT > 8 ? reinterpret_cast<const void*>(&k_paged_attn<T, D, true>)
                                 : reinterpret_cast<const void*>(&k_paged_attn<T, D, false>);
-  // per device and cheap: set on each call
-  NAB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedCfg<D>::kSmem));
+  static std::atomic<bool> ready[64][2];  // by device and variant; setting it twice does no harm
+  int dev = 0;
+  NAB_CUDA_CHECK(cudaGetDevice(&dev));
+  std::atomic<bool>& set = ready[dev & 63][p.GT > 8];
+  if (!set.load(std::memory_order_acquire)) {
+    NAB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedCfg<D>::kSmem));
+    set.store(true, std::memory_order_release);
+  }
   void* args[4] = {const_cast<CUtensorMap*>(&tk), const_cast<CUtensorMap*>(&tv), const_cast<CUtensorMap*>(&tq), &a};
   launch(kernel, dim3(p.grid), kPThreads, PagedCfg<D>::kSmem, s, args);
   if (p.join) {

@@ -4,6 +4,7 @@
 // device other than CUDA are refused last.
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/torch.h>
@@ -62,6 +63,12 @@ void check_pages(const char* op, const at::Tensor& k, const at::Tensor& v, at::S
   if (k.is_cuda()) at::assert_no_overlap(k, v);
 }
 
+// An uninitialised tensor on the device of `like` (the call's device guard is set): the allocator without the
+// dispatcher, which is what a call of a few microseconds has to save.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 int sms_of(const at::Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at::Tensor& cached,
@@ -97,10 +104,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
   at::assert_no_overlap(block_tables, cached);
   at::assert_no_overlap(block_tables, free_pages);
   const at::cuda::CUDAGuard guard(cached.device());
-  at::Tensor positions = at::empty({num_tokens}, cached.options());
-  at::Tensor slots = at::empty({num_tokens}, cached.options().dtype(at::kLong));
-  at::Tensor lengths = at::empty({B}, cached.options());
-  at::Tensor taken_out = at::empty({1}, cached.options());
+  at::Tensor positions = fresh({num_tokens}, at::kInt, cached), slots = fresh({num_tokens}, at::kLong, cached);
+  at::Tensor lengths = fresh({B}, at::kInt, cached), taken_out = fresh({1}, at::kInt, cached);
   nab::AssignPagesArgs a{};
   a.cached = cached.const_data_ptr<int>();
   a.starts = query_start ? query_start->const_data_ptr<int>() : nullptr;
@@ -121,21 +126,24 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
   return {positions, slots, lengths, taken_out};
 }
 
-void rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
-                       const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages, at::Tensor& v_pages,
-                       const OptTensor& q_norm, const OptTensor& k_norm, at::Tensor& out, double eps,
-                       bool interleaved) {
+// out: null for a new tensor
+at::Tensor rope_append_paged_to(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+                                const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
+                                at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
+                                double eps, bool interleaved, const at::Tensor* given) {
   constexpr const char* op = "rope_append_paged";
   const int dtype = half_dtype(op, qkv, "qkv");
   check_pages(op, k_pages, v_pages, qkv.scalar_type());
-  const int64_t Hkv = k_pages.size(1), P = k_pages.size(2), D = k_pages.size(3);
-  TORCH_CHECK(out.dim() == 3 && out.is_contiguous() && out.size(1) >= 1 && out.size(2) == D &&
-                  out.scalar_type() == qkv.scalar_type() && aligned16(out),
-              op, ": out must be contiguous [tokens, q_heads, ", D, "] of qkv's type");
-  const int64_t T = out.size(0), Hq = out.size(1);
-  TORCH_CHECK(Hq % Hkv == 0, op, ": ", Hq, " query heads do not divide over ", Hkv, " kv heads");
-  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == T && qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1, op,
-              ": qkv must be [", T, ", ", (Hq + 2 * Hkv) * D, "] with contiguous rows");
+  const int64_t Hkv = k_pages.size(1), P = k_pages.size(2), D = k_pages.size(3), Hq = q_heads;
+  TORCH_CHECK(Hq >= 1 && Hq < (1 << 20) && Hq % Hkv == 0, op, ": ", Hq, " query heads do not divide over ", Hkv,
+              " kv heads");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1, op, ": qkv must be [tokens, ",
+              (Hq + 2 * Hkv) * D, "] with contiguous rows");
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(given == nullptr || (given->dim() == 3 && given->size(0) == T && given->size(1) == Hq &&
+                                   given->size(2) == D && given->is_contiguous() &&
+                                   given->scalar_type() == qkv.scalar_type() && aligned16(*given)),
+              op, ": out must be contiguous [", T, ", ", Hq, ", ", D, "] of qkv's type");
   TORCH_CHECK(aligned16(qkv) && qkv.stride(0) % 8 == 0, op, ": the rows of qkv must be 16-byte aligned");
   TORCH_CHECK(cos.dim() == 2 && cos.is_contiguous() && sin.is_contiguous() && sin.sizes() == cos.sizes() &&
                   cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.size(0) >= 1,
@@ -159,9 +167,10 @@ void rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::T
                      {"v_pages", &v_pages},
                      {"q_norm", q_norm ? &*q_norm : nullptr},
                      {"k_norm", k_norm ? &*k_norm : nullptr},
-                     {"out", &out}});
-  at::assert_no_overlap(out, qkv);
+                     {"out", given}});
+  if (given) at::assert_no_overlap(*given, qkv);
   const at::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor out = given ? *given : fresh({T, Hq, D}, qkv.scalar_type(), qkv);
   nab::RopeAppendArgs a{};
   a.qkv = qkv.const_data_ptr();
   a.qkv_stride = qkv.stride(0);
@@ -184,10 +193,28 @@ void rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::T
   a.max_pos = static_cast<int>(cos.size(0));
   a.eps = static_cast<float>(eps);
   nab::rope_append_paged(at::cuda::getCurrentCUDAStream().stream(), a, dtype, interleaved);
+  return out;
 }
 
-void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                     const at::Tensor& block_tables, const at::Tensor& lengths, at::Tensor& out, double scale) {
+at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+                             const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
+                             at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
+                             double eps, bool interleaved) {
+  return rope_append_paged_to(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
+                              interleaved, nullptr);
+}
+
+void rope_append_paged_out(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+                           const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
+                           at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
+                           double eps, bool interleaved, at::Tensor& out) {
+  rope_append_paged_to(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps, interleaved,
+                       &out);
+}
+
+at::Tensor paged_attention_to(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                              const at::Tensor& block_tables, const at::Tensor& lengths, double scale,
+                              const at::Tensor* given) {
   constexpr const char* op = "paged_attention";
   const int dtype = half_dtype(op, q, "q");
   check_pages(op, k_pages, v_pages, q.scalar_type());
@@ -198,8 +225,8 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   TORCH_CHECK(q.stride(2) == 1 && (Hq == 1 || q.stride(1) == D) && aligned16(q) &&
                   (B <= 1 || (q.stride(0) >= Hq * D && q.stride(0) % D == 0)),
               op, ": the heads of q must be contiguous and 16-byte aligned, its rows a multiple of head_dim apart");
-  TORCH_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() &&
-                  aligned16(out),
+  TORCH_CHECK(given == nullptr || (given->sizes() == q.sizes() && given->is_contiguous() &&
+                                   given->scalar_type() == q.scalar_type() && aligned16(*given)),
               op, ": out must be contiguous, of q's shape and type");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == B && block_tables.scalar_type() == at::kInt &&
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
@@ -211,10 +238,11 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
                      {"v_pages", &v_pages},
                      {"block_tables", &block_tables},
                      {"lengths", &lengths},
-                     {"out", &out}});
-  at::assert_no_overlap(out, q);
-  if (B == 0) return;
+                     {"out", given}});
+  if (given) at::assert_no_overlap(*given, q);
   const at::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = given ? *given : fresh({B, Hq, D}, q.scalar_type(), q);
+  if (B == 0) return out;
   const int sms = sms_of(q);
   nab::PagedAttnArgs a{};
   a.q = q.const_data_ptr();
@@ -234,10 +262,20 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   a.D = static_cast<int>(D);
   a.scale = static_cast<float>(scale);
   // of this call alone: two streams or graphs never share it
-  const at::Tensor ws = at::empty({nab::paged_attention_ws_floats(a.B, a.M, a.P, a.Hq, a.Hkv, a.D, sms)},
-                                  q.options().dtype(at::kFloat));
+  const at::Tensor ws = fresh({nab::paged_attention_ws_floats(a.B, a.M, a.P, a.Hq, a.Hkv, a.D, sms)}, at::kFloat, q);
   a.ws = ws.mutable_data_ptr<float>();
   nab::paged_attention(at::cuda::getCurrentCUDAStream().stream(), a, dtype, sms);
+  return out;
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& block_tables, const at::Tensor& lengths, double scale) {
+  return paged_attention_to(q, k_pages, v_pages, block_tables, lengths, scale, nullptr);
+}
+
+void paged_attention_out(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                         const at::Tensor& block_tables, const at::Tensor& lengths, double scale, at::Tensor& out) {
+  paged_attention_to(q, k_pages, v_pages, block_tables, lengths, scale, &out);
 }
 
 using LogprobsResult = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
@@ -261,10 +299,9 @@ LogprobsResult token_logprobs(const at::Tensor& logits, const at::Tensor& tokens
   TORCH_CHECK(vocab_start >= 0, op, ": vocab_start must not be negative");
   check_devices(op, {{"logits", &logits}, {"tokens", &tokens}});
   const at::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  at::Tensor logprob = at::empty({rows}, f32), entropy = at::empty({rows}, f32), lse = at::empty({rows}, f32);
-  at::Tensor top_logprobs = at::empty({rows, top_k}, f32), top_tokens = at::empty({rows, top_k}, tokens.options());
-  at::Tensor top_logits = at::empty({rows, top_k}, f32);
+  at::Tensor logprob = fresh({rows}, at::kFloat, logits), entropy = fresh({rows}, at::kFloat, logits);
+  at::Tensor lse = fresh({rows}, at::kFloat, logits), top_logprobs = fresh({rows, top_k}, at::kFloat, logits);
+  at::Tensor top_tokens = fresh({rows, top_k}, at::kLong, logits), top_logits = fresh({rows, top_k}, at::kFloat, logits);
   nab::LogprobsArgs a{};
   a.logits = logits.const_data_ptr();
   a.stride = logits.stride(0);
@@ -291,11 +328,18 @@ TORCH_LIBRARY_FRAGMENT(nab, m) {
         "int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor)");
   m.impl("assign_pages", torch::dispatch(any, TORCH_FN(assign_pages)));
   m.def("rope_append_paged(Tensor qkv, Tensor cos, Tensor sin, Tensor positions, Tensor slots, Tensor(a!) k_pages, "
-        "Tensor(b!) v_pages, Tensor? q_norm, Tensor? k_norm, Tensor(c!) out, float eps, bool interleaved) -> ()");
+        "Tensor(b!) v_pages, int q_heads, Tensor? q_norm, Tensor? k_norm, float eps, bool interleaved) -> Tensor");
   m.impl("rope_append_paged", torch::dispatch(any, TORCH_FN(rope_append_paged)));
+  m.def("rope_append_paged.out(Tensor qkv, Tensor cos, Tensor sin, Tensor positions, Tensor slots, "
+        "Tensor(a!) k_pages, Tensor(b!) v_pages, int q_heads, Tensor? q_norm, Tensor? k_norm, float eps, "
+        "bool interleaved, Tensor(c!) out) -> ()");
+  m.impl("rope_append_paged.out", torch::dispatch(any, TORCH_FN(rope_append_paged_out)));
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, "
-        "Tensor(a!) out, float scale) -> ()");
+        "float scale) -> Tensor");
   m.impl("paged_attention", torch::dispatch(any, TORCH_FN(paged_attention)));
+  m.def("paged_attention.out(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, "
+        "float scale, Tensor(a!) out) -> ()");
+  m.impl("paged_attention.out", torch::dispatch(any, TORCH_FN(paged_attention_out)));
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k, int vocab_start) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.impl("token_logprobs", torch::dispatch(any, TORCH_FN(token_logprobs)));

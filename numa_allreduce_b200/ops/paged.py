@@ -63,7 +63,8 @@ def assign_pages(cached: torch.Tensor, block_tables: torch.Tensor, free_pages: t
         if query_start is not None:
             raise ValueError("assign_pages needs num_tokens with query_start")
         num_tokens = cached.shape[0]
-    r = PageSlots(*ops.assign_pages(cached, query_start, block_tables, free_pages, taken, page_size, num_tokens))
+    r = PageSlots(*ops.assign_pages.default(cached, query_start, block_tables, free_pages, taken, page_size,
+                                            num_tokens))
     after_launch()
     return r
 
@@ -91,10 +92,11 @@ def rope_append_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
     """
     ops = _ext.load()
     if out is None:
-        out = torch.empty(qkv.shape[0], q_heads, k_pages.shape[-1], dtype=qkv.dtype, device=qkv.device)
-    elif out.dim() != 3 or out.shape[1] != q_heads:
-        raise ValueError(f"rope_append_paged: out must be [tokens, {q_heads}, head_dim]")
-    ops.rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_norm, k_norm, out, eps, interleaved)
+        out = ops.rope_append_paged.default(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm,
+                                            eps, interleaved)
+    else:
+        ops.rope_append_paged.out(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
+                                  interleaved, out)
     after_launch()
     return out
 
@@ -117,10 +119,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     requests may be mixed; parts of a request are joined in a second launch.
     """
     ops = _ext.load()
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ops.paged_attention(q, k_pages, v_pages, block_tables, lengths, out,
-                        1.0 / math.sqrt(q.shape[-1]) if scale is None else scale)
+        out = ops.paged_attention.default(q, k_pages, v_pages, block_tables, lengths, scale)
+    else:
+        ops.paged_attention.out(q, k_pages, v_pages, block_tables, lengths, scale, out)
     after_launch()
     return out
 
