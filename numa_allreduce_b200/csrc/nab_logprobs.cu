@@ -7,13 +7,14 @@
 //   top k: by value, equal values by the lowest index
 //
 // One pass over the row with a running (m, S, sum) per thread, so each logit
-// is read from HBM once. The top k cost no second pass over the row: along
-// with its maximum each thread keeps the first piece (16 bytes) that held
-// it. Order the threads by (maximum, piece): an element of the top k can only
-// lie in the k first threads, because each thread before its own holds an
-// element that precedes it. The k-th of these keys is found by bisection
-// (block-wide counts), the pieces of k threads are read again (from L2),
-// elements that can precede it are collected in shared memory and ranked by
+// is read from HBM once. The top k cost no second pass over the row: each
+// thread notes, for each eighth of its share, the maximum and the first
+// 16-byte piece that held it. Take any partition of the row and order its
+// parts by (maximum, piece): an element of the top k can only lie in a part
+// whose key reaches the k-th of these keys, since each part before it holds
+// an element that precedes it. The k-th of 64 coarse parts is a cut; the
+// eighths that reach it (about 1.2 k of them) are read again, from L2, and
+// the elements that reach it are collected in shared memory and ranked by
 // counting. If a contrived row overflows the collection, k rounds of a block
 // maximum over the same pieces replace it.
 //
@@ -25,7 +26,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <stdexcept>
 #include <string>
 
@@ -38,10 +38,12 @@ namespace nab {
 
 namespace {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 1024;  // collected elements of a CTA
+constexpr int kSub = 8;      // parts of a thread's share
+constexpr int kCoarse = 64;  // parts that give the cut: the threads of one remainder mod 64
 constexpr float kL2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -149,15 +151,20 @@ struct Piece<__half> {
   }
 };
 
-// S = sum exp(x - m) and U = sum log2(e) (x - m) exp(x - m) for m >= every x
-// so far (m >= -FLT_MAX).
+// m: the largest value so far. With e(x) = log2(e) x - l, l = scaled_max(m):
+// s = sum 2^e(x), u = sum e(x) 2^e(x). One fused multiply-add gives e(x), and
+// the rounding of l cancels, since lse = (l + log2 s) / log2(e) uses the same.
 struct Stats {
   float m, s, u;
 };
+// Values below kFloor count as probability 0 and those above kCeil overflow:
+// a row whose maximum lies out there is summed again in another form.
+constexpr float kFloor = -1e38f, kCeil = 2e38f;
+// (a rounded product of its own: fused into a difference, equal maxima would not cancel)
+NAB_DINLINE float scaled_max(float m) { return __fmul_rn(fmaxf(m, kFloor), kL2e); }
 // exponents below -1000 count as -1000 (exp2 of them is zero), which keeps 0 * inf out
-NAB_DINLINE float exponent(float from, float to) { return fmaxf((from - to) * kL2e, -1000.f); }
 NAB_DINLINE void raise(Stats& a, float m) {
-  const float d = exponent(a.m, m), f = lp_ex2(d);
+  const float d = fmaxf(scaled_max(a.m) - scaled_max(m), -1000.f), f = lp_ex2(d);
   a.u = f * (a.u + d * a.s);
   a.s *= f;
   a.m = m;
@@ -165,27 +172,38 @@ NAB_DINLINE void raise(Stats& a, float m) {
 
 struct LpShared {
   float warp_m[kLpWarps], warp_s[kLpWarps], warp_u[kLpWarps];
-  Stats stats;                    // this CTA's, read by the cluster's first CTA
-  uint64_t top[kMaxTopK];         // this CTA's largest keys, in order; 0 past its elements
+  Stats stats;                          // this CTA's, read by the cluster's first CTA
+  uint64_t top[kMaxTopK];               // this CTA's largest keys, in order; 0 past its elements
   uint64_t cand[kCand];
-  uint64_t best[kLpWarps];
-  int who[kLpThreads];            // threads whose pieces are read again
+  float2 part[kSub * kLpThreads];       // of each part: its maximum, and as bits the first piece that holds it
+  uint64_t best[kLpThreads];            // (value, piece) of each thread's largest, 0 without pieces
+  uint64_t coarse[kCoarse];
+  int coarse_rank[kCoarse];
+  uint64_t cut;
+  int who[kSub * kLpThreads];           // parts that are read again
   int n_who, n_cand;
 };
 
-// A cut with at least k threads' keys at or above it (0 if fewer than k keys
-// are above 0), found bit by bit from `bits` down. Any such cut is right; it
-// ends once no more than `slack` threads too many are left.
-NAB_DINLINE uint64_t cut_of(uint64_t key, int k, int bits, int slack) {
-  if (__syncthreads_count(key != 0) < k) return 0;
-  uint64_t t = 0;
-  for (int bit = bits - 1; bit >= 0; --bit) {
-    const uint64_t c = t | (uint64_t{1} << bit);
-    const int n = __syncthreads_count(key >= c);
-    if (n >= k) t = c;
-    if (n >= k && n <= k + slack) break;
+// Sum over the block, for every thread, in a fixed order; a and b are used again after the next barrier.
+NAB_DINLINE float2 block_sum(float2 v, float* a, float* b) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  return t;
+  if (lane == 0) {
+    a[warp] = v.x;
+    b[warp] = v.y;
+  }
+  __syncthreads();
+  v = lane < kLpWarps ? make_float2(a[lane], b[lane]) : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
 }
 
 // A row as pieces of 16 aligned bytes: piece p holds the elements
@@ -231,24 +249,35 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   // Piece p is thread (p - p0) % kLpThreads's. Batches of kBatch pieces, the
   // next one's loads in flight during one's arithmetic; pieces past the end
   // read as -inf, which adds exactly nothing.
-  float m = -FLT_MAX, kv = -INFINITY;  // kv: the largest value so far, first held by piece kp
-  int kp = p0 + tid;
+  const int batches = ((p1 - p0 + kLpThreads - 1) / kLpThreads + kBatch - 1) / kBatch;
+  const int sub_batches = max(1, (batches + kSub - 1) / kSub);
+  // (value, piece within the CTA), larger = earlier, in as few bits as it takes
+  const int piece_bits = 32 - __clz(p1 - p0);
+  auto piece_key = [&](float x, int q) {
+    return (static_cast<uint64_t>(ordered(x) >> Piece<T>::kDrop) << piece_bits) | static_cast<uint64_t>(p1 - 1 - q);
+  };
+  float big = -INFINITY;  // largest value so far, first held by piece big_at
+  float kv = -INFINITY;   // the same within this part
   uint64_t s2 = 0, u2 = 0;
+  float l = scaled_max(big);
   const uint64_t l2e = pair(kL2e, kL2e);
-  auto fetch = [&](int p, uint4 (&w)[kBatch]) {
+  const uint4 fill = make_uint4(Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill);
+  const uint4* at = reinterpret_cast<const uint4*>(r.x - r.mis) + p0 + tid;  // aligned; piece 0 may begin before x
+  int p = p0 + tid, kp = p, big_at = p, sub = 0, left = sub_batches;
+  uint4 cur[kBatch];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    const int q = p + b * kLpThreads;
+    cur[b] = q >= i0 && q < i1 ? at[b * kLpThreads] : fill;
+  }
+  for (int j = 0; j < batches; ++j) {
+    uint4 next[kBatch];
+    at += kBatch * kLpThreads;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      w[b] = make_uint4(Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill);
-      if (p + b * kLpThreads < i1) w[b] = r.whole(p + b * kLpThreads);
+      next[b] = fill;
+      if (p + (kBatch + b) * kLpThreads < i1) next[b] = at[b * kLpThreads];
     }
-  };
-  int p = p0 + tid;
-  if (p < i0) p += kLpThreads;
-  uint4 cur[kBatch];
-  fetch(p, cur);
-  while (p < i1) {
-    uint4 next[kBatch];
-    fetch(p + kBatch * kLpThreads, next);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const float mx = Piece<T>::largest(cur[b]);
@@ -258,21 +287,21 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       }
     }
     {
-      const float to = fmaxf(m, kv);
-      const float d = exponent(m, to), f = lp_ex2(d);
+      const float to = fmaxf(l, __fmul_rn(kv, kL2e));
+      const float d = fmaxf(l - to, -1000.f), f = lp_ex2(d);
       const uint64_t f2 = pair(f, f);
       u2 = mul2(f2, fma2(pair(d, d), s2, u2));
       s2 = mul2(f2, s2);
-      m = to;
+      l = to;
     }
-    const uint64_t neg = pair(-m, -m);
+    const uint64_t neg = pair(-l, -l);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       uint64_t v[N / 2];
       Piece<T>::pairs(cur[b], v);
 #pragma unroll
       for (int e = 0; e < N / 2; ++e) {
-        const float2 d = unpair(mul2(add2(v[e], neg), l2e));
+        const float2 d = unpair(fma2(v[e], l2e, neg));
         const float d0 = max_nan(d.x, -1000.f), d1 = max_nan(d.y, -1000.f);
         const uint64_t w = pair(lp_ex2(d0), lp_ex2(d1));
         s2 = add2(s2, w);
@@ -282,22 +311,34 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) cur[b] = next[b];
     p += kBatch * kLpThreads;
+    if (--left == 0 || j + 1 == batches) {  // the end of a part
+      sh.part[sub * kLpThreads + tid] = make_float2(kv, __int_as_float(kp));
+      if (kv > big) {
+        big = kv;
+        big_at = kp;
+      }
+      kv = -INFINITY;
+      kp = p;
+      ++sub;
+      left = sub_batches;
+    }
   }
+  const int subs = sub;
   const float2 s_ = unpair(s2), u_ = unpair(u2);
-  Stats st = {m, s_.x + s_.y, u_.x + u_.y};
+  Stats st = {big, s_.x + s_.y, u_.x + u_.y};
   // the row's first and last piece, where they reach past it
   auto edge = [&](int q) {
     if (q < p0 || q >= p1 || r.inner(q) || (q - p0) % kLpThreads != tid) return;
+    float2& part_max = sh.part[(q - p0) / kLpThreads / kBatch / sub_batches * kLpThreads + tid];
     for (int e = 0; e < N; ++e) {
       const int i = r.first(q) + e;
       if (i < 0 || i >= a.V) continue;
       const float x = static_cast<float>(r.x[i]);
-      if (x > kv || (x == kv && q < kp)) {
-        kv = x;
-        kp = q;
-      }
+      if (x > part_max.x || (x == part_max.x && q < __float_as_int(part_max.y)))
+        part_max = make_float2(x, __int_as_float(q));
+      if (x > st.m || (x == st.m && q < big_at)) big_at = q;
       if (x > st.m) raise(st, x);
-      const float d = max_nan((x - st.m) * kL2e, -1000.f), w = lp_ex2(d);
+      const float d = max_nan(fmaf(x, kL2e, -scaled_max(st.m)), -1000.f), w = lp_ex2(d);
       st.s += w;
       st.u += d * w;
     }
@@ -305,60 +346,70 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   edge(0);
   if (pieces > 1) edge(pieces - 1);
 
-  // ------------------------------------------------ statistics of the CTA --
+  // ------------------------- statistics of the CTA, and the cut for its top k --
   float top = st.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) sh.warp_m[warp] = top;
+  sh.best[tid] = p0 + tid < p1 ? piece_key(st.m, big_at) : 0;
   if (tid < kMaxTopK) sh.top[tid] = 0;
-  if (tid == 0) sh.n_who = sh.n_cand = 0;
+  if (tid < kCoarse) sh.coarse_rank[tid] = 0;
+  if (tid == 0) {
+    sh.n_who = sh.n_cand = 0;
+    sh.cut = 0;
+  }
   __syncthreads();
+  if (tid < kCoarse) {
+    uint64_t c = 0;
+#pragma unroll
+    for (int i = 0; i < kLpThreads / kCoarse; ++i) {
+      const uint64_t b = sh.best[tid + i * kCoarse];
+      c = b > c ? b : c;
+    }
+    sh.coarse[tid] = c;
+  }
   top = sh.warp_m[lane % kLpWarps];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   raise(st, top);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
-    st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
-  }
-  if (lane == 0) {
-    sh.warp_s[warp] = st.s;
-    sh.warp_u[warp] = st.u;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    float s = lane < kLpWarps ? sh.warp_s[lane] : 0.f, u = lane < kLpWarps ? sh.warp_u[lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      u += __shfl_xor_sync(0xffffffffu, u, o);
-    }
-    if (lane == 0) sh.stats = {top, s, u};
-  }
+  const float2 sums = block_sum(make_float2(st.s, st.u), sh.warp_s, sh.warp_u);
+  if (tid == 0) sh.stats = {top, sums.x, sums.y};
 
   // ------------------------------------------------------ top k of the CTA --
   if (k > 0) {
-    // (value, piece within the CTA), larger = earlier, in as few bits as it takes
-    const int piece_bits = 32 - __clz(p1 - p0);
-    auto piece_key = [&](float x, int q) {
-      return (static_cast<uint64_t>(ordered(x) >> Piece<T>::kDrop) << piece_bits) |
-             static_cast<uint64_t>(p1 - 1 - q);
-    };
-    const bool has = p0 + tid < p1;
-    const uint64_t key = has ? piece_key(kv, kp) : 0;
-    const uint64_t cut = cut_of(key, k, 32 - Piece<T>::kDrop + piece_bits, 12);
-    if (has && key >= cut) sh.who[atomicAdd(&sh.n_who, 1)] = tid;
+    {
+      constexpr int kEach = kCoarse * kCoarse / kLpThreads;  // comparisons of a thread
+      const int i = tid % kCoarse, from = tid / kCoarse * kEach;
+      const uint64_t mine = sh.coarse[i];
+      int before = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) before += sh.coarse[from + j] > mine;
+      if (before) atomicAdd(&sh.coarse_rank[i], before);
+    }
+    __syncthreads();
+    // the k-th; if fewer than k coarse parts hold anything, the cut stays 0
+    if (tid < kCoarse && sh.coarse_rank[tid] == k - 1 && sh.coarse[tid] != 0) sh.cut = sh.coarse[tid];
+    __syncthreads();
+    const uint64_t cut = sh.cut;
+    for (int i = 0; i < subs; ++i) {
+      const float2 part_max = sh.part[i * kLpThreads + tid];
+      const int q = __float_as_int(part_max.y);
+      if (q < p1 && piece_key(part_max.x, q) >= cut) sh.who[atomicAdd(&sh.n_who, 1)] = i * kLpThreads + tid;
+    }
     __syncthreads();
     const int n_who = sh.n_who;
-    const int depth = (p1 - p0 + kLpThreads - 1) / kLpThreads;  // pieces of a thread, at most
+    const int depth = kBatch * sub_batches;  // pieces of a part, at most
+    const uint32_t cut_value = static_cast<uint32_t>(cut >> piece_bits);
     auto for_elements = [&](auto f) {
       for (int i = tid; i < n_who * depth; i += kLpThreads) {
-        const int q = p0 + sh.who[i / depth] + (i % depth) * kLpThreads;
+        const int part_at = sh.who[i / depth];
+        const int q = p0 + part_at % kLpThreads + (part_at / kLpThreads * depth + i % depth) * kLpThreads;
         if (q >= p1) continue;
         if (r.inner(q)) {
+          const uint4 w = r.whole(q);
+          if ((ordered(Piece<T>::largest(w)) >> Piece<T>::kDrop) < cut_value) continue;
           Acc<T> v;
-          acc_set(v, r.whole(q));
+          acc_set(v, w);
 #pragma unroll
           for (int e = 0; e < N; ++e)
             if (piece_key(v.v[e], q) >= cut) f(key_of(v.v[e], static_cast<uint32_t>(r.first(q) + e)));
@@ -386,20 +437,20 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
     } else {
       uint64_t last = ~uint64_t{0};
       for (int i = 0; i < k; ++i) {
-        uint64_t best = 0;
+        uint64_t next = 0;
         for_elements([&](uint64_t x) {
-          if (x < last && x > best) best = x;
+          if (x < last && x > next) next = x;
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-          const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
-          best = b > best ? b : best;
+          const uint64_t b = __shfl_xor_sync(0xffffffffu, next, o);
+          next = b > next ? b : next;
         }
-        if (lane == 0) sh.best[warp] = best;
+        if (lane == 0) sh.best[warp] = next;
         __syncthreads();
-        for (int w = 0; w < kLpWarps; ++w) best = sh.best[w] > best ? sh.best[w] : best;
-        if (tid == 0) sh.top[i] = best;
-        last = best;
+        for (int w = 0; w < kLpWarps; ++w) next = sh.best[w] > next ? sh.best[w] : next;
+        if (tid == 0) sh.top[i] = next;
+        last = next;
         __syncthreads();
       }
     }
@@ -420,6 +471,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
         all.m = fmaxf(all.m, part_[c].m);
       }
       // keys of every CTA, one per thread (8 x 32 at most); all are different
+      static_assert(kMaxCluster * kMaxTopK <= kLpThreads && kMaxCluster * kMaxTopK <= kCand, "one key per thread");
       if (tid < cluster * k) {
         const uint32_t at = sm100::dsmem_addr(sm100::smem_u32(&sh.top[tid % k]), tid / k);
         const uint32_t lo = __float_as_uint(sm100::ld_dsmem_f32(at)), hi = __float_as_uint(sm100::ld_dsmem_f32(at + 4));
@@ -437,12 +489,31 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
     } else if (tid < k) {
       mine = sh.top[tid];
     }
-    const float log2_s = log2f(all.s);
+    // a row whose largest finite value is out of reach of the scaled form: this CTA sums it again as it stands
+    const bool far = all.m > kCeil || all.m < kFloor;
+    if (far && fabsf(all.m) != INFINITY) {
+      float2 sum = make_float2(0.f, 0.f);
+      for (int i = tid; i < a.V; i += kLpThreads) {
+        const float d = max_nan((static_cast<float>(r.x[i]) - all.m) * kL2e, -1000.f), w = lp_ex2(d);
+        sum.x += w;
+        sum.y += d * w;
+      }
+      __syncthreads();
+      sum = block_sum(sum, sh.warp_s, sh.warp_u);
+      all.s = sum.x;
+      all.u = sum.y;
+    }
+    const float log2_s = log2f(all.s), scaled = scaled_max(all.m);
+    const float lse = far ? all.m + log2_s * kLn2 : (scaled + log2_s) * kLn2;
+    auto logprob_of = [&](float x) {
+      if (far) return (x - all.m) - log2_s * kLn2;
+      return x < kFloor ? x - lse : (fmaf(x, kL2e, -scaled) - log2_s) * kLn2;
+    };
     if (tid == 0) {
       const int64_t at = a.tokens[row] - a.vocab_start;
       const bool here = at >= 0 && at < a.V;
-      a.logprob[row] = here ? (picked - all.m) - log2_s * kLn2 : -INFINITY;
-      a.lse[row] = all.m + log2_s * kLn2;
+      a.logprob[row] = here ? logprob_of(picked) : -INFINITY;
+      a.lse[row] = lse;
       a.entropy[row] = (log2_s - all.u / all.s) * kLn2;
     }
     if (mine != 0) {
@@ -453,7 +524,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       }
       if (rank < k) {
         const float x = unordered(static_cast<uint32_t>(mine >> 32));
-        a.top_logprobs[row * k + rank] = (x - all.m) - log2_s * kLn2;
+        a.top_logprobs[row * k + rank] = logprob_of(x);
         a.top_logits[row * k + rank] = x;
         a.top_tokens[row * k + rank] = static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(mine)) + a.vocab_start;
       }
@@ -464,9 +535,13 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
 
 template <typename T>
 void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
-  // CTAs per row: as many as keep two per SM busy, each with at least 2048 elements
+  // CTAs per row. A cluster pays for its two barriers and its slower launch, so only rows of many bytes and few
+  // of them are shared: at least 30 KB of logits per CTA, at most two CTAs per SM. Measured with 1 / 2 / 4 / 8
+  // CTAs per row (us, k = 20): 1 x 128256 bf16 12.2 / 10.1 / 8.1 / 7.7; 64 rows 18.0 / 13.7 / 11.6 / 16.1; 148 rows
+  // 18.7 / 16.1 / 18.7 / 26.5; 300 rows 26.0 / 26.6 / 31.7 / 49.0; 1 x 16032 5.4 / 5.9 / 6.1 / 6.9.
   int cluster = 1;
-  while (cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * sms && a.V / (cluster * 2) >= 2048) cluster *= 2;
+  const int64_t bytes = static_cast<int64_t>(a.V) * sizeof(T);
+  while (cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * sms && bytes / (cluster * 2) >= 30 * 1024) cluster *= 2;
   cudaLaunchConfig_t cfg{};
   const int64_t grid = a.rows * cluster;
   if (grid > 0x7fffffff) throw std::invalid_argument("token_logprobs: too many rows for one launch");
