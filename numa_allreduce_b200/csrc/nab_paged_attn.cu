@@ -12,25 +12,37 @@
 // kernel of nab_attn_sm100.cu), a serial chain that costs more than the
 // bytes of a chunk; here four warps stream independently.
 //
-// Work: the (request, kv head, head tile) segments, cut into tiles of 64
-// positions, laid end to end and dealt out in equal contiguous ranges to a
-// grid of two CTAs per SM, so that ragged batches and single long requests
-// load the GPU alike. Lengths are read on the device (a captured graph
-// replays at any lengths); each CTA finds its range from a scan over them. A
-// segment that lies in one CTA is written at once; of a segment that is cut,
-// each CTA leaves (max, sum, unnormalised output) in fp32 and a second
-// launch joins the parts in order.
+// Work: the (request, kv head, head tile) segments, cut into tiles of 32 KB
+// of K and V (64 positions of 128 dims, 128 of 64). Lengths are read on the
+// device: a captured graph replays at any lengths. Three ways to deal the
+// tiles out, chosen on the host from the table's width (plan_of):
+//   even     all tiles laid end to end, equal contiguous ranges for a grid of
+//            two CTAs per SM, so that ragged batches and single long requests
+//            load the GPU alike. Each CTA finds its range by a scan over the
+//            lengths. A segment within one CTA is written at once; of a cut
+//            one, each CTA leaves (max, sum, unnormalised output) in fp32 and
+//            a second launch joins the parts in order. (Joining in the CTA
+//            that finds all parts written needs no second launch but takes
+//            longer: two fences, a read of the flags and the join, 3 to 5 us
+//            that hold up the CTA's next segment, against 2.3 us.)
+//   whole    the same with ranges of whole segments, for short requests: no
+//            part, no second launch.
+//   cluster  calls bound by latency: a thread-block cluster of 1 to 8 CTAs
+//            per segment, joined over distributed shared memory, without
+//            scan, workspace or second launch.
 //
-// CTA: warp 4 produces, warps 0-3 consume. A tile arrives as TMA boxes of 16
-// rows x 64 dims (128-byte swizzle), one per producer lane, looked up in the
-// block table box by box (any page size that is a multiple of 16). Warp w takes rows [16w, 16w + 16) of
-// each tile with its own running maximum and sum, so the warps meet only at
-// the end of a segment.
+// CTA: warp 4 fetches, warps 0-3 compute. A tile arrives as TMA boxes of 64
+// dims x as many rows as the page size allows (16 to a whole tile, 128-byte
+// swizzle): issuing one takes its warp about 60 cycles whatever its size (16
+// boxes of 2 KB are 900 cycles, 4 of 8 KB 260). The tile that holds a
+// request's end is fetched in boxes of 16 rows, no further than it goes.
+// Warp w computes a quarter of each tile with its own running maximum and
+// sum, so the warps meet only at the end of a segment.
 //
 // Every mbarrier wait is bounded. One that runs out records into the device's
-// kernel error record; the CTA's warps then walk their ranges without
-// waiting or computing (the same barriers), the producer waits (bounded) for
-// its copies in flight, and the kernel returns.
+// kernel error record; the warps then walk their ranges without waiting,
+// fetching or computing (the same barriers), the fetching warp waits
+// (bounded) for its copies in flight, and the kernel returns.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,6 +53,7 @@
 #include <cstring>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "nab_device.cuh"
 #include "nab_driver.h"
@@ -52,19 +65,22 @@ namespace nab {
 
 namespace {
 
-constexpr int kTile = 64;       // positions per stage
-constexpr int kBoxRows = 16;    // rows of one TMA box: one consumer warp's share of a tile
-constexpr int kConsumers = 4;   // consumer warps
-constexpr int kPThreads = 32 * (kConsumers + 1);
+constexpr int kBoxRows = 16;    // rows of the smallest TMA box, and of one step of a warp
+constexpr int kWarps = 4;       // computing warps
+constexpr int kPThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;       // query heads of one head tile (the MMA's M)
 constexpr int kJoinThreads = 256;
+constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
 struct PagedCfg {
-  static constexpr int kBoxBytes = kBoxRows * D * 2;
-  static constexpr int kStageBytes = 2 * (kTile / kBoxRows) * kBoxBytes;  // K boxes, then V boxes
-  static constexpr int kStages = 96 * 1024 / kStageBytes;                 // 3 (D = 128), 6 (D = 64)
+  static constexpr int kTile = 8192 / D;                       // positions of a tile
+  static constexpr int kSteps = kTile / kWarps / kBoxRows;     // 16-row steps of a warp's share: 1 (D = 128), 2 (D = 64)
+  static constexpr int kHalves = D / 64;                       // 128-byte column blocks of a row
+  static constexpr int kBlock = kTile * 128;                   // bytes of one column block of a tile
+  static constexpr int kStageBytes = 2 * kHalves * kBlock;     // K blocks, then V blocks: 32 KB
+  static constexpr int kStages = 3;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kMergeBytes = 2 * 8 * D * 4;  // two warps' partial of 8 rows
   static constexpr int kQ = kStages * kStageBytes;   // two buffers behind the ring
@@ -80,20 +96,21 @@ struct PagedDev {
   int64_t table_stride;
   const int* lengths;
   void* out;
-  float* ws_o;    // [2 * grid][16][D]
-  float2* ws_ml;  // [2 * grid][16]
-  int4* desc;     // [grid]: the cut segment that begins in a CTA (row, heads, last CTA, 1), or w = 0
+  float* ws_o;    // [2 * grid][16][D]: parts
+  float2* ws_ml;  // [2 * grid][16]: their (max, sum)
+  int4* desc;     // [grid]: the cut segment that begins in a CTA (output row, heads, last CTA, 1 + inside), or w = 0
   int num_pages;
   int B, M, P, Hq, Hkv;
   int G;          // query heads per kv head
   int HT, GT;     // head tiles per kv head, heads per tile
+  int cluster;    // CTAs per segment (cluster form)
+  int whole;      // ranges of whole segments
+  int box_rows;   // rows of the large boxes
   float scale_log2;
   ErrorState* err;
   uint32_t* err_host;
   uint64_t timeout_ns;
 };
-
-NAB_DINLINE void bar_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory"); }
 
 NAB_DINLINE void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -150,12 +167,15 @@ NAB_DINLINE float ex2(float x) {
 
 NAB_DINLINE int64_t min64(int64_t x, int64_t y) { return x < y ? x : y; }
 
-// A walk over the segments of one CTA's range [x, x1) of tiles.
+NAB_DINLINE void bar_compute() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+// A walk over the segments of one CTA's range [x, x1): tiles, all segments
+// end to end (even, cluster), or segments (whole).
 struct Walk {
-  int x, x1;     // next tile, end of the range (in tiles, all segments end to end)
+  int x, x1;
   int b, h;      // request, kv head * HT + head tile
   int nt, len;   // tiles and positions of request b
-  int t0;        // first tile of the current piece within the segment
+  int t;         // next tile within the segment
 };
 
 // Length of request b, within what its table row can hold.
@@ -163,20 +183,22 @@ NAB_DINLINE int length_of(const PagedDev& a, int b) {
   return static_cast<int>(min64(max(a.lengths[b], 0), static_cast<int64_t>(a.M) * a.P));
 }
 
-template <typename T, int D, bool kWide>
+// kWide: more than 8 heads in a head tile. kCluster: the cluster form.
+template <typename T, int D, bool kWide, bool kCluster>
 __global__ void __launch_bounds__(kPThreads, 2)
     k_paged_attn(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                 const __grid_constant__ CUtensorMap tk16, const __grid_constant__ CUtensorMap tv16,
                  const __grid_constant__ CUtensorMap tq, const __grid_constant__ PagedDev a) {
   using C = PagedCfg<D>;
   constexpr int S = C::kStages;
-  constexpr int kHalves = D / 64;            // 128-byte column blocks of a row
-  constexpr int kHalfBytes = kBoxRows * 128;  // of a K or V box, and of a Q buffer
+  constexpr int kTile = C::kTile, kSteps = C::kSteps, kHalves = C::kHalves;
+  constexpr int kQHalf = kRows * 128;  // one column block of a Q buffer
   extern __shared__ __align__(1024) uint8_t paged_smem[];
   const uint32_t base = sm100::smem_u32(paged_smem);
   uint64_t* full = reinterpret_cast<uint64_t*>(paged_smem + C::kBars);
   uint64_t* empty = full + S;
   uint64_t* q_empty = empty + S;
-  int* misc = reinterpret_cast<int*>(paged_smem + C::kMisc);  // abort, b, first tile of b, total tiles, warp sums
+  int* misc = reinterpret_cast<int*>(paged_smem + C::kMisc);  // abort, b, first unit of b, -, warp sums
   volatile int* abort_flag = misc;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int HH = a.Hkv * a.HT;
@@ -188,10 +210,10 @@ __global__ void __launch_bounds__(kPThreads, 2)
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       sm100::mbar_init(&full[s], 1);
-      sm100::mbar_init(&empty[s], kConsumers);
+      sm100::mbar_init(&empty[s], kWarps);
     }
-    sm100::mbar_init(&q_empty[0], kConsumers);
-    sm100::mbar_init(&q_empty[1], kConsumers);
+    sm100::mbar_init(&q_empty[0], kWarps);
+    sm100::mbar_init(&q_empty[1], kWarps);
     sm100::fence_barrier_init();
     misc[0] = 0;
     misc[1] = a.B;
@@ -202,152 +224,319 @@ __global__ void __launch_bounds__(kPThreads, 2)
   pdl_wait();
   pdl_trigger();
 
-  // Scan of the requests' tile counts: thread i holds the requests
-  // [i * per_thread, ...), then a block scan.
-  const int per_thread = (a.B + kPThreads - 1) / kPThreads;
-  const int rb0 = min(a.B, tid * per_thread), rb1 = min(a.B, rb0 + per_thread);
-  int mine = 0;
-  for (int b = rb0; b < rb1; ++b) {
-    const int raw = a.lengths[b];
-    if (blockIdx.x == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
-      record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(b));
-    mine += (length_of(a, b) + kTile - 1) / kTile;
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) misc[4 + warp] = incl;
-  __syncthreads();
-  int before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kPThreads / 32; ++w) {
-    before += w < warp ? misc[4 + w] : 0;
-    total += misc[4 + w];
-  }
-  const int W = total * HH;
-  const int per = max(1, (W + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  const int64_t lo64 = static_cast<int64_t>(blockIdx.x) * per;
-  const int lo = static_cast<int>(min64(lo64, W)), hi = static_cast<int>(min64(lo64 + per, W));
-  // the request that holds tile `lo`
-  if (lo < hi && before * HH <= lo && lo < (before + mine) * HH) {
-    int cum = before;
-    for (int b = rb0; b < rb1; ++b) {
-      const int nt = (length_of(a, b) + kTile - 1) / kTile;
-      if (lo < (cum + nt) * HH) {
-        misc[1] = b;
-        misc[2] = cum;
-        break;
-      }
-      cum += nt;
-    }
-  }
-  __syncthreads();
   Walk w;
-  w.x = lo;
-  w.x1 = hi;
-  w.b = misc[1];
-  w.h = 0;
-  w.nt = 0;
-  w.len = 0;
-  w.t0 = 0;
-  if (lo < hi) {
+  int per = 1, lo = 0;  // units per CTA, first unit of this one's range
+  if constexpr (kCluster) {
+    const int segment = static_cast<int>(blockIdx.x) / a.cluster, rank = static_cast<int>(blockIdx.x) % a.cluster;
+    w.b = segment / HH;
+    w.h = segment % HH;
+    const int raw = a.lengths[w.b];
+    if (tid == 0 && rank == 0 && w.h == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
+      record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(w.b));
     w.len = length_of(a, w.b);
     w.nt = (w.len + kTile - 1) / kTile;
-    const int y = lo - misc[2] * HH;
-    w.h = y / w.nt;
-    w.t0 = y - w.h * w.nt;
+    const int share = (w.nt + a.cluster - 1) / a.cluster;
+    w.t = min(w.nt, rank * share);
+    w.x = 0;
+    w.x1 = min(w.nt, w.t + share) - w.t;
+    __syncthreads();  // barriers initialised
+  } else {
+    // Scan of the requests' units (tiles, or 1 if there is any): thread i
+    // holds the requests [i * per_thread, ...), then a block scan.
+    const int per_thread = (a.B + kPThreads - 1) / kPThreads;
+    const int rb0 = min(a.B, tid * per_thread), rb1 = min(a.B, rb0 + per_thread);
+    auto units = [&](int b) {
+      const int len = length_of(a, b);
+      return a.whole ? (len > 0) : (len + kTile - 1) / kTile;
+    };
+    int mine = 0;
+    for (int b = rb0; b < rb1; ++b) {
+      const int raw = a.lengths[b];
+      if (blockIdx.x == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
+        record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(b));
+      mine += units(b);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) misc[4 + warp] = incl;
+    __syncthreads();
+    int before = incl - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < kPThreads / 32; ++i) {
+      before += i < warp ? misc[4 + i] : 0;
+      total += misc[4 + i];
+    }
+    const int W = total * HH;
+    per = max(1, (W + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int64_t lo64 = static_cast<int64_t>(blockIdx.x) * per;
+    lo = static_cast<int>(min64(lo64, W));
+    const int hi = static_cast<int>(min64(lo64 + per, W));
+    // the request that holds unit `lo`
+    if (lo < hi && before * HH <= lo && lo < (before + mine) * HH) {
+      int cum = before;
+      for (int b = rb0; b < rb1; ++b) {
+        const int n = units(b);
+        if (lo < (cum + n) * HH) {
+          misc[1] = b;
+          misc[2] = cum;
+          break;
+        }
+        cum += n;
+      }
+    }
+    __syncthreads();
+    w.x = lo;
+    w.x1 = hi;
+    w.b = misc[1];
+    w.h = 0;
+    w.nt = 0;
+    w.len = 0;
+    w.t = 0;
+    if (lo < hi) {
+      w.len = length_of(a, w.b);
+      w.nt = (w.len + kTile - 1) / kTile;
+      const int y = lo - misc[2] * HH, n = a.whole ? 1 : w.nt;
+      w.h = y / n;
+      w.t = y - w.h * n;
+    }
   }
-  auto next_segment = [&]() {
-    w.t0 = 0;
-    if (++w.h < HH) return;
+  // tiles of the current segment in this range, and the step to the next one
+  auto tiles_here = [&]() { return !kCluster && a.whole ? w.nt : min(w.nt - w.t, w.x1 - w.x); };
+  auto advance = [&](int n) -> bool {
+    w.x += !kCluster && a.whole ? 1 : n;
+    if (w.x >= w.x1) return false;
+    w.t = 0;
+    if (++w.h < HH) return true;
     w.h = 0;
     do {
       ++w.b;
       w.len = w.b < a.B ? length_of(a, w.b) : 1;
     } while (w.len == 0);
     w.nt = (w.len + kTile - 1) / kTile;
+    return true;
   };
   auto fail = [&](uint32_t observed) {
     if (!*abort_flag) record_local_failure(a.err, a.err_host, kErrTimeout, kStageAttn, observed);
     *abort_flag = 1;
   };
 
-  if (warp == kConsumers) {
-    // --------------------------------------------------------- producer --
-    // lane -> (K or V, warp share of the tile, 64-dim column block): one TMA box each
-    constexpr int kBoxes = 2 * (kTile / kBoxRows) * kHalves;
+  if (warp == kWarps) {
+    // -------------------------------------------------------- fetching --
+    // Lane -> one box of a tile: (K or V, column block, run of rows).
     int tile = 0, seg = 0;
-    const CUtensorMap* map = lane < kBoxes / 2 ? &tk : &tv;
-    const int half = lane % kHalves, box = (lane / kHalves) % (kTile / kBoxRows);
-    const int64_t bad_row = static_cast<int64_t>(a.num_pages) * a.Hkv * a.P;  // past the pages: TMA fills zeros
-    auto row_of = [&](int t) -> int64_t {  // first cache row of this lane's box of tile t
-      const int pos = t * kTile + box * kBoxRows;
-      if (lane >= kBoxes || pos >= w.len) return -1;
-      const int page = __ldg(a.tables + w.b * a.table_stride + pos / a.P);
-      if (page < 0 || page >= a.num_pages) {
-        if (lane < kBoxes / 2 && half == 0 && w.h == 0)
-          record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(page));
-        return bad_row;
-      }
-      return (static_cast<int64_t>(page) * a.Hkv + w.h / a.HT) * a.P + pos % a.P;
+    // lane i holds the id of page window + i of request w.b, and of page i of request w.b + 1, loaded when the walk
+    // comes to w.b so that the next request starts without a wait
+    int window = 0, ids = 0, ahead = 0;
+    auto load_ids = [&](int b, int first) {
+      return b < a.B && first + lane < a.M ? __ldg(a.tables + b * a.table_stride + first + lane) : 0;
     };
-    while (w.x < w.x1) {
-      const int n = min(w.nt - w.t0, w.x1 - w.x);
-      int64_t row = row_of(w.t0);
+    bool more = w.x < w.x1, given_up = false;
+    if (more) {
+      window = static_cast<int>(static_cast<int64_t>(w.t) * kTile / a.P);
+      ids = load_ids(w.b, window);
+      ahead = load_ids(w.b + 1, 0);
+    }
+    while (more) {
+      const int n = tiles_here();
+      const int kvh = w.h / a.HT;
       for (int i = 0; i < n; ++i, ++tile) {
         const int s = tile % S;
-        const int64_t row_next = i + 1 < n ? row_of(w.t0 + i + 1) : -1;
-        if (!*abort_flag && tile >= S && !sm100::mbar_wait(&empty[s], (tile / S - 1) & 1, a.timeout_ns, abort_flag))
-          fail(tile);
-        if (i == 0 && !*abort_flag && seg >= 2 &&
-            !sm100::mbar_wait(&q_empty[seg & 1], (seg / 2 - 1) & 1, a.timeout_ns, abort_flag))
-          fail(tile);
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-        const int boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
-        if (lane == 0)
-          sm100::mbar_arrive_expect_tx(&full[s], boxes * kHalfBytes + (i == 0 ? C::kQBytes : 0));
+        const int left = w.len - (w.t + i) * kTile;  // positions from this tile on
+        const bool small = left < kTile;
+        const int rows = small ? kBoxRows : a.box_rows;
+        const int per_block = kTile / rows;          // boxes of a column block
+        const int v = lane / (kHalves * per_block), half = lane / per_block % kHalves, from = lane % per_block * rows;
+        const bool mine = v < 2 && from < left;
+        const int pos = (w.t + i) * kTile + (mine ? from : 0);
+        const int page_at = pos / a.P, first = (w.t + i) * kTile / a.P;
+        if (first < window || first + kTile / kBoxRows > window + 32) {  // a tile has at most kTile / 16 pages
+          window = first;
+          ids = load_ids(w.b, window);
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, page_at - window);
+        int64_t row = (static_cast<int64_t>(page) * a.Hkv + kvh) * a.P + (pos - page_at * a.P);
+        if (page < 0 || page >= a.num_pages) {
+          if (mine && v == 0 && half == 0 && w.h == 0)
+            record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(page));
+          row = static_cast<int64_t>(a.num_pages) * a.Hkv * a.P;  // past the pages: TMA fills zeros
+        }
+        const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+        bool ok = tile < S || sm100::mbar_wait(&empty[s], (tile / S - 1) & 1, a.timeout_ns, abort_flag);
+        if (ok && i == 0 && seg >= 2) ok = sm100::mbar_wait(&q_empty[seg & 1], (seg / 2 - 1) & 1, a.timeout_ns, abort_flag);
+        if (!ok) fail(tile);
+        if (__any_sync(0xffffffffu, !ok)) {
+          given_up = true;
+          break;
+        }
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&full[s], boxes * rows * 128 + (i == 0 ? C::kQBytes : 0));
         __syncwarp();
         if (i == 0 && lane < kHalves)
-          tma_load_3d(paged_smem + C::kQ + (seg & 1) * C::kQBytes + half * kHalfBytes, &tq, half * 64,
-                      (w.h / a.HT) * a.G + (w.h % a.HT) * a.GT, w.b, &full[s]);
-        if (row >= 0)
-          sm100::tma_load_2d(paged_smem + s * C::kStageBytes + lane * kHalfBytes, map, half * 64,
-                             static_cast<int>(row), &full[s]);
-        row = row_next;
+          tma_load_3d(paged_smem + C::kQ + (seg & 1) * C::kQBytes + lane * kQHalf, &tq, lane * 64,
+                      kvh * a.G + (w.h % a.HT) * a.GT, w.b, &full[s]);
+        if (mine)
+          sm100::tma_load_2d(paged_smem + s * C::kStageBytes + (v * kHalves + half) * C::kBlock + from * 128,
+                             small ? (v ? &tv16 : &tk16) : (v ? &tv : &tk), half * 64, static_cast<int>(row), &full[s]);
       }
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-      w.x += n;
+      if (given_up) break;
       ++seg;
-      if (w.x < w.x1) next_segment();
+      const int b = w.b;
+      more = advance(n);
+      if (more && w.b != b) {
+        ids = w.b == b + 1 ? ahead : load_ids(w.b, 0);
+        window = 0;
+        ahead = load_ids(w.b + 1, 0);
+      }
     }
-    // the copies in flight land before the CTA's memory goes away, whatever the consumers do
+    // the copies in flight land before the CTA's memory goes away, whatever the other warps do
     volatile int never = 0;
     for (int i = max(0, tile - S); i < tile; ++i)
       sm100::mbar_wait(&full[i % S], (i / S) & 1, a.timeout_ns, &never);
+    if constexpr (kCluster) {
+      if (a.cluster > 1) {
+        sm100::cluster_sync();  // the parts are in shared memory
+        sm100::cluster_sync();  // and have been read
+      }
+    }
     return;
   }
 
-  // ------------------------------------------------------------ consumers --
-  // requests without positions: their rows are zero
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (length_of(a, b) > 0) continue;
-    uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.Hq * D);
-    for (int i = tid; i < a.Hq * D / 8; i += 32 * kConsumers) o[i] = make_uint4(0u, 0u, 0u, 0u);
+  // ----------------------------------------------------------- computing --
+  if constexpr (!kCluster) {
+    // requests without positions: their rows are zero
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (length_of(a, b) > 0) continue;
+      uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.Hq * D);
+      for (int i = tid; i < a.Hq * D / 8; i += 32 * kWarps) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (tid == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
-  if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 
   constexpr int kNt = D / 8;           // output column tiles
   constexpr int kR = kWide ? 2 : 1;    // row halves in use
   const int g = lane >> 2, t4 = lane & 3;
   const int lr = lane & 7, lm = lane >> 3;  // ldmatrix: row within a matrix, matrix
+  // Byte offsets of this lane's ldmatrix rows within a 16-row step, for column chunk 0 (16-byte chunks permuted by
+  // row % 8); column step j is 32 bytes on, i.e. XOR j << 5.
+  const uint32_t k_off = (warp * kSteps * kBoxRows + lr + (lm >> 1) * 8) * 128 + (((lm & 1) ^ lr) << 4);
+  const uint32_t v_off = (warp * kSteps * kBoxRows + lr + (lm & 1) * 8) * 128 + (((lm >> 1) ^ lr) << 4);
   uint32_t qf[D / 16][4];
   int tile = 0, seg = 0;
-  while (w.x < w.x1) {
-    const int n = min(w.nt - w.t0, w.x1 - w.x);
-    float acc[kNt][4], m[kR], l[kR];
+  bool dead = false;
+  // a segment's running maximum, sum and output of this warp's positions
+  float acc[kNt][4], m[kR], l[kR];
+
+  // One tile's share: nv valid rows, all of them unless kTail.
+  auto compute = [&](uint32_t stage, int nv, auto tail) {
+    constexpr bool kTail = decltype(tail)::value;
+    const uint32_t kb = stage + k_off, vb = stage + C::kStageBytes / 2 + v_off;
+    // scores: two chains of products per 8 positions (even and odd 16-dim steps) while there is one step of rows
+    constexpr int kChains = kSteps == 1 ? 2 : 1;
+    float sc[2 * kSteps][4], odd[2][4];
+#pragma unroll
+    for (int j = 0; j < 2 * kSteps; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) odd[j][0] = odd[j][1] = odd[j][2] = odd[j][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x) {
+        // matrices: (positions 0-7 | 8-15 by lm >> 1) x (dims 0-7 | 8-15 by lm & 1)
+        uint32_t kf[4];
+        ldsm4((kb ^ ((k & 3) << 5)) + (k >> 2) * C::kBlock + x * kBoxRows * 128, kf);
+        if (kChains == 2 && (k & 1)) {
+          mma16816<T>(odd[0], qf[k], kf[0], kf[1]);
+          mma16816<T>(odd[1], qf[k], kf[2], kf[3]);
+        } else {
+          mma16816<T>(sc[2 * x], qf[k], kf[0], kf[1]);
+          mma16816<T>(sc[2 * x + 1], qf[k], kf[2], kf[3]);
+        }
+      }
+    }
+    if (kChains == 2) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] += odd[j][e];
+      }
+    }
+    uint32_t pf[kSteps][4];
+    bool grown = false;
+    float alpha[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      float v[4 * kSteps];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4 * kSteps; ++e) {
+        v[e] = sc[e >> 1][2 * r + (e & 1)] * a.scale_log2;
+        if (kTail && (e >> 1) * 8 + 2 * t4 + (e & 1) >= nv) v[e] = -INFINITY;
+        mx = fmaxf(mx, v[e]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx);
+      grown |= mn != m[r];
+      // every score -inf so far: subtract 0, so that exp(-inf) = 0 and no NaN comes from inf - inf
+      const float ms = mn == -INFINITY ? 0.f : mn;
+      alpha[r] = ex2(m[r] - ms);
+      m[r] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4 * kSteps; ++e) {
+        v[e] = ex2(v[e] - ms);
+        sum += v[e];
+      }
+      l[r] = l[r] * alpha[r] + sum;
+      // rounded to 16 bits for the product with V, as V itself is; the sum keeps 32
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x) {
+        pf[x][r] = pack2<T>(v[4 * x], v[4 * x + 1]);
+        pf[x][2 + r] = pack2<T>(v[4 * x + 2], v[4 * x + 3]);
+      }
+    }
+    if (!kWide) {
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x) pf[x][1] = pf[x][3] = 0u;
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          acc[j][2 * r] *= alpha[r];
+          acc[j][2 * r + 1] *= alpha[r];
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      // rows past the length may hold anything (NaN too): zero them in the fragments
+      const int p0 = x * kBoxRows + 2 * t4, p1 = p0 + 8;
+      const uint32_t mask0 = (p0 < nv ? 0xffffu : 0u) | (p0 + 1 < nv ? 0xffff0000u : 0u);
+      const uint32_t mask1 = (p1 < nv ? 0xffffu : 0u) | (p1 + 1 < nv ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        // matrices: (positions 0-7 | 8-15 by lm & 1) x (dims 0-7 | 8-15 by lm >> 1), transposed
+        uint32_t vf[4];
+        ldsm4_t((vb ^ ((j & 3) << 5)) + (j >> 2) * C::kBlock + x * kBoxRows * 128, vf);
+        if (kTail) {
+          vf[0] &= mask0;
+          vf[1] &= mask1;
+          vf[2] &= mask0;
+          vf[3] &= mask1;
+        }
+        mma16816<T>(acc[2 * j], pf[x], vf[0], vf[1]);
+        mma16816<T>(acc[2 * j + 1], pf[x], vf[2], vf[3]);
+      }
+    }
+  };
+
+  for (bool more = w.x < w.x1; more;) {
+    const int n = tiles_here(), t0 = w.t;
 #pragma unroll
     for (int j = 0; j < kNt; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
@@ -357,94 +546,29 @@ __global__ void __launch_bounds__(kPThreads, 2)
     }
     for (int i = 0; i < n; ++i, ++tile) {
       const int s = tile % S;
-      if (!*abort_flag && !sm100::mbar_wait(&full[s], (tile / S) & 1, a.timeout_ns, abort_flag)) fail(tile);
-      // the warp goes on together: a lane that gave up takes the others along
-      const bool dead = __any_sync(0xffffffffu, *abort_flag != 0);
-      if (!dead && i == 0) {
-        // Q fragments: A rows are heads; matrices (rows 0-7 | 8-15) x (dims 0-7 | 8-15) of each 16-dim step
-        const uint32_t qb = base + C::kQ + (seg & 1) * C::kQBytes;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const int row = lr + (lm & 1) * 8, chunk = (k & 3) * 2 + (lm >> 1);
-          ldsm4(qb + (k >> 2) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4), qf[k]);
-        }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&q_empty[seg & 1]);
+      // a lane that gave up takes the others along; once dead, the warp only keeps the barriers
+      if (!dead) {
+        const bool ok = sm100::mbar_wait(&full[s], (tile / S) & 1, a.timeout_ns, abort_flag);
+        if (!ok) fail(tile);
+        dead = __any_sync(0xffffffffu, !ok);
       }
-      const int nv = w.len - (w.t0 + i) * kTile - warp * kBoxRows;  // valid rows of this warp's box
-      if (!dead && nv > 0) {
-        const uint32_t kb = base + s * C::kStageBytes + warp * C::kBoxBytes;
-        const uint32_t vb = kb + (kTile / kBoxRows) * C::kBoxBytes;
-        float sc[2][4];
+      if (!dead) {
+        if (i == 0) {
+          // Q fragments: A rows are heads; matrices (rows 0-7 | 8-15) x (dims 0-7 | 8-15) of each 16-dim step
+          const uint32_t qb = base + C::kQ + (seg & 1) * C::kQBytes;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          // matrices: (positions 0-7 | 8-15 by lm >> 1) x (dims 0-7 | 8-15 by lm & 1)
-          const int row = lr + (lm >> 1) * 8, chunk = (k & 3) * 2 + (lm & 1);
-          uint32_t kf[4];
-          ldsm4(kb + (k >> 2) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4), kf);
-          mma16816<T>(sc[0], qf[k], kf[0], kf[1]);
-          mma16816<T>(sc[1], qf[k], kf[2], kf[3]);
-        }
-        uint32_t pf[4];
-        bool grown = false;
-        float alpha[kR];
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          float v[4] = {sc[0][2 * r] * a.scale_log2, sc[0][2 * r + 1] * a.scale_log2, sc[1][2 * r] * a.scale_log2,
-                        sc[1][2 * r + 1] * a.scale_log2};
-          if (nv < kBoxRows) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if ((e >> 1) * 8 + 2 * t4 + (e & 1) >= nv) v[e] = -INFINITY;
+          for (int k = 0; k < D / 16; ++k) {
+            const int row = lr + (lm & 1) * 8, chunk = (k & 3) * 2 + (lm >> 1);
+            ldsm4(qb + (k >> 2) * kQHalf + row * 128 + ((chunk ^ (row & 7)) << 4), qf[k]);
           }
-          float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[r], mx);
-          grown |= mn != m[r];
-          // every score -inf so far: subtract 0, so that exp(-inf) = 0 and no NaN comes from inf - inf
-          const float ms = mn == -INFINITY ? 0.f : mn;
-          alpha[r] = ex2(m[r] - ms);
-          m[r] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = ex2(v[e] - ms);
-            sum += v[e];
-          }
-          l[r] = l[r] * alpha[r] + sum;
-          // rounded to 16 bits for the product with V, as V itself is; the sum keeps 32
-          pf[r] = pack2<T>(v[0], v[1]);
-          pf[2 + r] = pack2<T>(v[2], v[3]);
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&q_empty[seg & 1]);
         }
-        if (!kWide) pf[1] = pf[3] = 0u;
-        if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-          for (int j = 0; j < kNt; ++j) {
-#pragma unroll
-            for (int r = 0; r < kR; ++r) {
-              acc[j][2 * r] *= alpha[r];
-              acc[j][2 * r + 1] *= alpha[r];
-            }
-          }
-        }
-        // rows past the length may hold anything (NaN too): zero them in the fragments
-        uint32_t mask0 = 0xffffffffu, mask1 = 0xffffffffu;
-        if (nv < kBoxRows) {
-          const int p0 = 2 * t4, p1 = p0 + 8;
-          mask0 = (p0 < nv ? 0xffffu : 0u) | (p0 + 1 < nv ? 0xffff0000u : 0u);
-          mask1 = (p1 < nv ? 0xffffu : 0u) | (p1 + 1 < nv ? 0xffff0000u : 0u);
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          // matrices: (positions 0-7 | 8-15 by lm & 1) x (dims 0-7 | 8-15 by lm >> 1), transposed
-          const int row = lr + (lm & 1) * 8, chunk = (j & 3) * 2 + (lm >> 1);
-          uint32_t vf[4];
-          ldsm4_t(vb + (j >> 2) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4), vf);
-          mma16816<T>(acc[2 * j], pf, vf[0] & mask0, vf[1] & mask1);
-          mma16816<T>(acc[2 * j + 1], pf, vf[2] & mask0, vf[3] & mask1);
+        const int nv = w.len - (t0 + i) * kTile - warp * kSteps * kBoxRows;  // valid rows of this warp's share
+        if (nv >= kSteps * kBoxRows) {
+          compute(base + s * C::kStageBytes, nv, std::false_type{});
+        } else if (nv > 0) {
+          compute(base + s * C::kStageBytes, nv, std::true_type{});
         }
       }
       __syncwarp();
@@ -478,7 +602,7 @@ __global__ void __launch_bounds__(kPThreads, 2)
             ml[2 * g + 1] = l[r];
           }
         }
-        bar_consumers();
+        bar_compute();
         if (takes) {
           const float mo_ = ml[2 * g], lo_ = ml[2 * g + 1];
           const float mn = fmaxf(m[r], mo_);
@@ -493,15 +617,27 @@ __global__ void __launch_bounds__(kPThreads, 2)
             acc[j][2 * r + 1] = acc[j][2 * r + 1] * w0 + o.y * w1;
           }
         }
-        if (step == 1) bar_consumers();  // the buffers are free again
+        if (step == 1) bar_compute();  // the buffers are free again
       }
     }
-    if (warp == 0) {
-      const bool whole = w.t0 == 0 && n == w.nt;
-      const int h0 = (w.h % a.HT) * a.GT;          // first head of the tile within the group
-      const int heads = min(a.GT, a.G - h0);
-      const int64_t row0 = static_cast<int64_t>(w.b) * a.Hq + (w.h / a.HT) * a.G + h0;
-      if (whole) {
+    const int h0 = (w.h % a.HT) * a.GT;  // first head of the tile within the group
+    const int heads = min(a.GT, a.G - h0);
+    const int64_t row0 = static_cast<int64_t>(w.b) * a.Hq + (w.h / a.HT) * a.G + h0;
+    if (kCluster && a.cluster > 1) {
+      // this CTA's part, for the cluster: [16][D] floats, then 16 x (max, sum), where the ring was
+      if (warp == 0) {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          const int row = g + 8 * r;
+          float* o = reinterpret_cast<float*>(paged_smem) + row * D + 2 * t4;
+#pragma unroll
+          for (int j = 0; j < kNt; ++j)
+            *reinterpret_cast<float2*>(o + 8 * j) = make_float2(acc[j][2 * r], acc[j][2 * r + 1]);
+          if (t4 == 0) reinterpret_cast<float2*>(paged_smem + kRows * D * 4)[row] = make_float2(m[r], l[r]);
+        }
+      }
+    } else if (warp == 0) {
+      if (t0 == 0 && n == w.nt) {
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
           const int row = g + 8 * r;
@@ -527,15 +663,66 @@ __global__ void __launch_bounds__(kPThreads, 2)
             if (t4 == 0) a.ws_ml[part * kRows + row] = make_float2(m[r], l[r]);
           }
         }
-        if (w.t0 == 0 && lane == 0) {
-          const int last = static_cast<int>((static_cast<int64_t>(w.x) + w.nt - 1) / per);  // CTA of the last tile
+        if (t0 == 0 && lane == 0) {
+          const int last = (w.x + w.nt - 1) / per;  // CTA of the last tile
           a.desc[blockIdx.x] = make_int4(static_cast<int>(row0), heads, last, 1 + (w.x != lo));
         }
       }
     }
-    w.x += n;
     ++seg;
-    if (w.x < w.x1) next_segment();
+    more = advance(n);
+  }
+  if constexpr (kCluster) {
+    if (a.cluster == 1) {
+      if (seg == 0) {  // a request without positions: zeros
+        const int h0 = (w.h % a.HT) * a.GT, heads = min(a.GT, a.G - h0);
+        uint2* o = reinterpret_cast<uint2*>(static_cast<T*>(a.out) +
+                                            (static_cast<int64_t>(w.b) * a.Hq + (w.h / a.HT) * a.G + h0) * D);
+        for (int i = tid; i < heads * (D / 4); i += 32 * kWarps) o[i] = make_uint2(0u, 0u);
+      }
+      return;
+    }
+    if (seg == 0 && tid < kRows)  // no tile for this CTA: a part of weight 0
+      reinterpret_cast<float2*>(paged_smem + kRows * D * 4)[tid] = make_float2(-INFINITY, 0.f);
+    sm100::cluster_sync();
+    const int h0 = (w.h % a.HT) * a.GT, heads = min(a.GT, a.G - h0);
+    const int rank = static_cast<int>(blockIdx.x) % a.cluster;
+    T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(w.b) * a.Hq + (w.h / a.HT) * a.G + h0) * D;
+    // the cluster's CTAs share the output in runs of 4 dims; parts in rank order
+    for (int i = rank * 32 * kWarps + tid; i < heads * (D / 4); i += a.cluster * 32 * kWarps) {
+      const uint32_t ml_at = base + kRows * D * 4 + i / (D / 4) * 8, o_at = base + i * 16;
+      float2 ml[kMaxCluster];
+      float4 x[kMaxCluster];
+      float M = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {
+        const int from = min(c, a.cluster - 1);
+        const uint32_t at = sm100::dsmem_addr(ml_at, from);
+        ml[c] = make_float2(sm100::ld_dsmem_f32(at), sm100::ld_dsmem_f32(at + 4));
+        x[c] = sm100::ld_dsmem_f4(sm100::dsmem_addr(o_at, from));
+        M = fmaxf(M, ml[c].x);
+      }
+      const float ms = M == -INFINITY ? 0.f : M;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {
+        // a part without tiles has nothing stored but its (max, sum)
+        if (c >= a.cluster || (ml[c].x == -INFINITY && ml[c].y == 0.f)) continue;
+        const float wgt = ex2(ml[c].x - ms);
+        den += wgt * ml[c].y;
+        o.x += wgt * x[c].x;
+        o.y += wgt * x[c].y;
+        o.z += wgt * x[c].z;
+        o.w += wgt * x[c].w;
+      }
+      const float inv = w.len == 0 ? 0.f : 1.f / den;  // a request without positions: zeros
+      uint2 packed;
+      packed.x = pack2<T>(o.x * inv, o.y * inv);
+      packed.y = pack2<T>(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(out + static_cast<int64_t>(i) * 4) = packed;
+    }
+    sm100::cluster_sync();  // the others' shared memory has been read
   }
 }
 
@@ -624,11 +811,11 @@ CUtensorMap encode(const void* ptr, int dtype, int rank, const cuuint64_t* dims,
   return m;
 }
 
-// Pages as a matrix [rows, D]; a box is 16 rows of one 64-dim column block.
-CUtensorMap page_map(const void* ptr, int dtype, int64_t rows, int D) {
+// Pages as a matrix [rows, D]; a box is some rows of one 64-dim column block.
+CUtensorMap page_map(const void* ptr, int dtype, int64_t rows, int D, int box_rows) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(D) * 2};
-  const cuuint32_t box[2] = {64, kBoxRows};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
   return encode(ptr, dtype, 2, dims, strides, box);
 }
 
@@ -644,36 +831,57 @@ CUtensorMap q_map(const PagedAttnArgs& a, int dtype) {
 
 struct PagedPlan {
   int HT, GT, grid;
-  bool join;
+  int cluster;   // CTAs per segment in the cluster form, 0 for the others
+  bool whole;    // ranges of whole segments
+  int box_rows;
 };
 
-PagedPlan plan_of(int B, int M, int P, int Hq, int Hkv, int sms) {
+PagedPlan plan_of(int B, int M, int P, int Hq, int Hkv, int D, int sms) {
   PagedPlan p;
   const int G = Hq / Hkv;
   p.HT = (G + kRows - 1) / kRows;
   p.GT = (G + p.HT - 1) / p.HT;
-  const int64_t tiles = (static_cast<int64_t>(M) * P + kTile - 1) / kTile;  // of the longest request
-  const int64_t most = tiles * B * Hkv * p.HT;
-  if (most > 0x3fffffff) throw std::invalid_argument("paged_attention: too many positions for one call");
-  p.grid = static_cast<int>(std::min<int64_t>(2 * sms, std::max<int64_t>(1, most)));
-  p.join = tiles > 1;  // a request of one tile is never cut
+  const int tile = 8192 / D;
+  const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(M) * P + tile - 1) / tile);  // of the longest request
+  const int64_t segments = static_cast<int64_t>(B) * Hkv * p.HT, slots = 2 * sms;
+  if (tiles * segments > 0x3fffffff)
+    throw std::invalid_argument("paged_attention: too many positions for one call");
+  // The cluster form takes ceil(tiles / c) tiles one after the other, the even one ceil(tiles * segments / slots) and
+  // about three more for its second launch. Measured (us, cluster / even; 8 heads per kv head, D = 128): 1 request of
+  // 1025 6.8 / 6.8, of 4096 11.1 / 7.5; 32 of 2500 12.3 / 15.0; 128 of 1025 17.1 / 20.2. The bound of 10 tiles keeps
+  // ragged batches, where the longest request decides, from losing more than that.
+  int c = 1;
+  while (c < kMaxCluster && 2 * c <= tiles && segments * c * 2 <= slots) c *= 2;
+  const int64_t share = (tiles + c - 1) / c, even = (tiles * segments + slots - 1) / slots;
+  p.cluster = segments * c <= slots && share <= std::min<int64_t>(10, even + 3) ? c : 0;
+  // Short requests are not worth a cut: up to 4 tiles of imbalance against the second launch.
+  p.whole = !p.cluster && tiles <= 4;
+  p.grid = static_cast<int>(p.cluster ? segments * c : std::min<int64_t>(slots, p.whole ? segments : tiles * segments));
+  p.box_rows = tile;
+  while (P % p.box_rows != 0) p.box_rows /= 2;  // P is a multiple of 16
   return p;
 }
 
-// ws: [2 * grid][16][D] outputs, [2 * grid][16] (max, sum), [grid] descriptors
-int64_t ws_floats(int grid, int D) { return static_cast<int64_t>(grid) * (2 * kRows * (D + 2) + 4); }
+// ws: [2 * grid][16][D] outputs, [2 * grid][16] (max, sum), [grid] descriptors: for the even form alone
+int64_t ws_floats(const PagedPlan& p, int D) {
+  return p.cluster || p.whole ? 0 : static_cast<int64_t>(p.grid) * (2 * kRows * (D + 2) + 4);
+}
 
-void launch(const void* kernel, dim3 grid, int block, size_t smem, cudaStream_t s, void** args) {
+void launch(const void* kernel, dim3 grid, int block, size_t smem, int cluster, cudaStream_t s, void** args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
   if (e != cudaSuccess)
     throw std::runtime_error(std::string("paged_attention launch failed: ") + cudaGetErrorString(e));
@@ -681,9 +889,12 @@ void launch(const void* kernel, dim3 grid, int block, size_t smem, cudaStream_t 
 
 template <typename T, int D>
 void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
-  const PagedPlan p = plan_of(in.B, in.M, in.P, in.Hq, in.Hkv, sms);
+  const PagedPlan p = plan_of(in.B, in.M, in.P, in.Hq, in.Hkv, D, sms);
   const int64_t rows = in.num_pages * in.Hkv * in.P;
-  const CUtensorMap tk = page_map(in.k_pages, dtype, rows, D), tv = page_map(in.v_pages, dtype, rows, D);
+  const CUtensorMap tk16 = page_map(in.k_pages, dtype, rows, D, kBoxRows);
+  const CUtensorMap tv16 = page_map(in.v_pages, dtype, rows, D, kBoxRows);
+  const CUtensorMap tk = p.box_rows == kBoxRows ? tk16 : page_map(in.k_pages, dtype, rows, D, p.box_rows);
+  const CUtensorMap tv = p.box_rows == kBoxRows ? tv16 : page_map(in.v_pages, dtype, rows, D, p.box_rows);
   const CUtensorMap tq = q_map(in, dtype);
   const KernelErrorRecord rec = kernel_error_record();
   PagedDev a{};
@@ -694,6 +905,9 @@ void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
   a.ws_o = in.ws;
   a.ws_ml = reinterpret_cast<float2*>(in.ws + static_cast<int64_t>(p.grid) * 2 * kRows * D);
   a.desc = reinterpret_cast<int4*>(a.ws_ml + static_cast<int64_t>(p.grid) * 2 * kRows);
+  a.cluster = p.cluster;
+  a.whole = p.whole;
+  a.box_rows = p.box_rows;
   a.num_pages = static_cast<int>(in.num_pages);
   a.B = in.B;
   a.M = in.M;
@@ -707,28 +921,32 @@ void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
   a.err = rec.dev;
   a.err_host = rec.host;
   a.timeout_ns = kernel_timeout_ns();
-  const void* kernel = p.GT > 8 ? reinterpret_cast<const void*>(&k_paged_attn<T, D, true>)
-                                : reinterpret_cast<const void*>(&k_paged_attn<T, D, false>);
-  static std::atomic<bool> ready[64][2];  // by device and variant; setting it twice does no harm
+  const bool wide = p.GT > 8;
+  const void* kernel = p.cluster ? (wide ? reinterpret_cast<const void*>(&k_paged_attn<T, D, true, true>)
+                                         : reinterpret_cast<const void*>(&k_paged_attn<T, D, false, true>))
+                                 : (wide ? reinterpret_cast<const void*>(&k_paged_attn<T, D, true, false>)
+                                         : reinterpret_cast<const void*>(&k_paged_attn<T, D, false, false>));
+  static std::atomic<bool> ready[64][4];  // by device and variant; setting it twice does no harm
   int dev = 0;
   NAB_CUDA_CHECK(cudaGetDevice(&dev));
-  std::atomic<bool>& set = ready[dev & 63][p.GT > 8];
+  std::atomic<bool>& set = ready[dev & 63][2 * (p.cluster > 0) + wide];
   if (!set.load(std::memory_order_acquire)) {
     NAB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedCfg<D>::kSmem));
     set.store(true, std::memory_order_release);
   }
-  void* args[4] = {const_cast<CUtensorMap*>(&tk), const_cast<CUtensorMap*>(&tv), const_cast<CUtensorMap*>(&tq), &a};
-  launch(kernel, dim3(p.grid), kPThreads, PagedCfg<D>::kSmem, s, args);
-  if (p.join) {
-    void* jargs[1] = {&a};
-    launch(reinterpret_cast<const void*>(&k_paged_join<T, D>), dim3(p.grid, p.GT), kJoinThreads, 0, s, jargs);
+  void* args[6] = {const_cast<CUtensorMap*>(&tk),   const_cast<CUtensorMap*>(&tv), const_cast<CUtensorMap*>(&tk16),
+                   const_cast<CUtensorMap*>(&tv16), const_cast<CUtensorMap*>(&tq), &a};
+  launch(kernel, dim3(p.grid), kPThreads, PagedCfg<D>::kSmem, p.cluster, s, args);
+  if (!p.cluster && !p.whole) {
+    void* join_args[1] = {&a};
+    launch(reinterpret_cast<const void*>(&k_paged_join<T, D>), dim3(p.grid, p.GT), kJoinThreads, 0, 0, s, join_args);
   }
 }
 
 }  // namespace
 
 int64_t paged_attention_ws_floats(int B, int M, int P, int Hq, int Hkv, int D, int sms) {
-  return ws_floats(plan_of(B, M, P, Hq, Hkv, sms).grid, D);
+  return ws_floats(plan_of(B, M, P, Hq, Hkv, D, sms), D);
 }
 
 void paged_attention(cudaStream_t s, const PagedAttnArgs& a, int dtype, int sms) {
