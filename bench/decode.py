@@ -37,6 +37,8 @@ def parse():
     p.add_argument("--model", default="70b", choices=["70b", "8b", "tiny"])
     p.add_argument("--impls", default="fused,baseline")
     p.add_argument("--attention", default="tc", choices=["tc", "simt"])
+    p.add_argument("--kv", default="contiguous", choices=["contiguous", "paged"],
+                   help="paged: a pool of 64-row pages (assign_pages, rope_append_paged, paged_attention)")
     p.add_argument("--reps", type=int, default=20)
     p.add_argument("--shard-as", type=int, default=None,
                    help="single GPU: decode one rank's shard of an N-way TP model (no allreduce)")
@@ -86,9 +88,9 @@ def main():
     rows = []
     for B in [int(b) for b in args.batches.split(",")]:
         model = LlamaTPDecoder(cfg, comm, batch=B, context=args.context, shard_of=args.shard_as,
-                               attention=args.attention)
+                               attention=args.attention, kv=args.kv)
         model.tokens.copy_(torch.arange(B, device="cuda") * 7 + 3)
-        row = {"batch": B, "world_size": world, "context": args.context, "layers": cfg.layers,
+        row = {"batch": B, "world_size": world, "context": args.context, "layers": cfg.layers, "kv": args.kv,
                "weight_gb_per_rank": round(model.weight_bytes() / 1e9, 2)}
         finals = {}
         for impl in args.impls.split(","):

@@ -24,8 +24,9 @@ Public API (parity with the reference's ``src/__init__.py``, which exported
   :func:`rope_tables`: decode over a paged KV cache (block tables and slots on
   the GPU, head norm + rotation + append, split attention for requests of
   different lengths);
-* :func:`token_logprobs`, :func:`join_token_logprobs`: log-probabilities of
-  given tokens with entropy and top alternatives, per vocabulary shard;
+* :func:`token_logprobs`, :func:`join_token_logprobs`,
+  :func:`gather_token_logprobs`: log-probabilities of given tokens with
+  entropy and top alternatives, per vocabulary shard and joined over shards;
 * :class:`LlamaConfig`, :class:`LlamaTPDecoder`: the tensor-parallel decoder
   built on them (in ``numa_allreduce_b200.models``, imported lazily);
 * :class:`PeerMonitor`, :class:`PeerLost`: host-side failure detection;
@@ -36,7 +37,7 @@ Public API (parity with the reference's ``src/__init__.py``, which exported
 from .ops.errors import KernelError, check_kernels, reset_kernels
 from .ops.fused import fused_allreduce_rmsnorm, rmsnorm_residual
 from .ops.gemm import PackedWeight, gemm, gemm_allreduce_rmsnorm, gemm_swiglu, interleave_gate_up, pack_weight
-from .ops.logprobs import TokenLogprobs, join_token_logprobs, token_logprobs
+from .ops.logprobs import TokenLogprobs, gather_token_logprobs, join_token_logprobs, token_logprobs
 from .ops.paged import PageSlots, assign_pages, paged_attention, rope_append_paged, rope_tables
 from .parallel.comm import AllReduceError, NumaAwareAllReduce
 from .parallel.emulate import emulate_all_gather, emulate_allreduce, emulate_reduce_scatter
@@ -66,6 +67,7 @@ __all__ = [
     "emulate_allreduce",
     "emulate_reduce_scatter",
     "fused_allreduce_rmsnorm",
+    "gather_token_logprobs",
     "gemm",
     "gemm_allreduce_rmsnorm",
     "gemm_swiglu",

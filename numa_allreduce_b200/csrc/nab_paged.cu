@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) k_rope_append_paged(const __grid_constant
   if (rotated) {
     int pos = a.positions[t];
     if (pos < 0 || pos >= a.max_pos) {
-      if (live && is_q && h0 == 0 && c == 0)
+      if (live && is_q && h0 == 0 && c == 0 && a.slots[t] >= 0)  // a token without a slot is dropped anyway
         record_local_failure(p.err, p.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(t));
       pos = min(max(pos, 0), a.max_pos - 1);
     }

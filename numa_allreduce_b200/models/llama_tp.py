@@ -22,6 +22,12 @@ both variants: the baseline as separate RoPE/KV-append and attention
 launches, the fused variant as one launch that does both. Weights are random N(0, 0.02) (there is no
 checkpoint), the KV cache random N(0, 1); every buffer a step touches is
 static so the whole step is captured in one CUDA graph.
+
+With ``kv="paged"`` the cache is a pool of pages and every request has its own
+length: a step gives the new tokens their pages (``assign_pages``), appends
+with ``rope_append_paged`` and attends with ``paged_attention``;
+:meth:`LlamaTPDecoder.advance` makes its tokens the next step's, so a captured
+step + advance decodes token after token.
 """
 
 from __future__ import annotations
@@ -37,6 +43,8 @@ from ..ops import _ext
 from ..ops.errors import check_enabled, check_kernels
 from ..ops.fused import fused_allreduce_rmsnorm, rmsnorm_residual
 from ..ops.gemm import gemm, gemm_allreduce_rmsnorm, gemm_swiglu, interleave_gate_up, pack_weight
+from ..ops.logprobs import TokenLogprobs, gather_token_logprobs, token_logprobs
+from ..ops.paged import PageSlots, assign_pages, paged_attention, rope_append_paged, rope_tables
 
 
 @dataclass
@@ -92,12 +100,32 @@ class LlamaTPDecoder:
         attention: ``"tc"`` for the tensor-core decode attention (tcgen05
             scores and output per 128-position chunk), ``"simt"`` for the
             SIMT kernel; the fused variant only (the baseline uses the
-            two-launch SIMT path).
+            two-launch SIMT path). Contiguous cache only.
+        kv: ``"contiguous"``, or ``"paged"``: a pool of pages, for both
+            variants.
+        lengths: tokens already in the cache of each request (paged only;
+            default ``context`` for all).
+        page_size: rows of a page (paged only).
+        max_new: tokens per request that the pool has room for beyond
+            ``lengths`` (paged only).
+        logprobs: with a number, each step also leaves the new tokens'
+            log-probabilities, entropies and that many top alternatives in
+            ``self.logprobs`` (:class:`~numa_allreduce_b200.TokenLogprobs`).
     """
 
     def __init__(self, cfg: LlamaConfig, comm, batch: int, context: int, impl: str = "fused", seed: int = 0,
                  device: torch.device | str = "cuda", attn_splits: int | None = None, shard_of: int | None = None,
-                 attention: str = "tc"):
+                 attention: str = "tc", kv: str = "contiguous", lengths: list[int] | None = None,
+                 page_size: int = 64, max_new: int = 1, logprobs: int | None = None):
+        if kv not in ("contiguous", "paged"):
+            raise ValueError("kv must be 'contiguous' or 'paged'")
+        if kv == "contiguous" and lengths is not None:
+            raise ValueError("lengths needs kv='paged'")
+        if kv == "paged" and (page_size < 16 or page_size % 16 or max_new < 1):
+            raise ValueError("kv='paged' needs a page_size that is a multiple of 16 and max_new >= 1")
+        lengths = [context] * batch if lengths is None else [int(n) for n in lengths]
+        if len(lengths) != batch or min(lengths) < 0:
+            raise ValueError("lengths must hold one length per request")
         if impl not in ("fused", "baseline"):
             raise ValueError("impl must be 'fused' or 'baseline'")
         self.cfg, self.comm, self.impl = cfg, comm, impl
@@ -116,7 +144,15 @@ class LlamaTPDecoder:
         self.tp = W
         self.I = cfg.intermediate // W
         self.B, self.ctx = batch, context
-        self.Lmax = _round_up(context + 1, 64)
+        self.kv, self.page_size = kv, page_size
+        if kv == "paged":
+            held = [-(-n // page_size) for n in lengths]
+            width = [-(-(n + max_new) // page_size) for n in lengths]
+            self.Lmax = max(width) * page_size
+            cache_shape = (sum(width), self.Hkv, page_size, D)
+        else:
+            self.Lmax = _round_up(context + 1, 64)
+            cache_shape = (batch, self.Hkv, self.Lmax, D)
         H = cfg.hidden
         g = torch.Generator(device=self.device).manual_seed(1234 + self.rank + 7919 * seed)
 
@@ -130,10 +166,8 @@ class LlamaTPDecoder:
                 "wqkv": w(qkv_rows, H), "wo": w(H, self.Hq * D), "wgu": w(2 * self.I, H), "wd": w(H, self.I),
                 "in_norm": torch.ones(H, device=self.device, dtype=torch.bfloat16),
                 "post_norm": torch.ones(H, device=self.device, dtype=torch.bfloat16),
-                "k": torch.randn(batch, self.Hkv, self.Lmax, D, generator=g, device=self.device,
-                                 dtype=torch.bfloat16),
-                "v": torch.randn(batch, self.Hkv, self.Lmax, D, generator=g, device=self.device,
-                                 dtype=torch.bfloat16),
+                "k": torch.randn(cache_shape, generator=g, device=self.device, dtype=torch.bfloat16),
+                "v": torch.randn(cache_shape, generator=g, device=self.device, dtype=torch.bfloat16),
             })
         gv = torch.Generator(device=self.device).manual_seed(4321 + 7919 * seed)  # replicated tables
         self.embed = torch.randn(cfg.vocab, H, generator=gv, device=self.device, dtype=torch.bfloat16) * 0.02
@@ -144,10 +178,7 @@ class LlamaTPDecoder:
         # contiguous 16 KB block of HBM per weight tile); built on first use
         # of the fused path
         self._packed: dict[tuple[int, str], object] = {}
-        # rotary tables
-        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, device=self.device, dtype=torch.float64) / D))
-        ang = torch.arange(self.Lmax, device=self.device, dtype=torch.float64)[:, None] * inv[None, :]
-        self.cos, self.sin = ang.cos().float().contiguous(), ang.sin().float().contiguous()
+        self.cos, self.sin = rope_tables(self.Lmax, D, theta=cfg.rope_theta, device=self.device)
         # static step buffers
         bf = dict(device=self.device, dtype=torch.bfloat16)
         self.tokens = torch.zeros(batch, device=self.device, dtype=torch.long)
@@ -168,6 +199,26 @@ class LlamaTPDecoder:
         self.splits_tc = attn_splits or int(self.ops.attention_splits_tc(batch, self.Hkv, context + 1))
         self.gemm_splits = {}
         self.next_tokens = torch.zeros(batch, device=self.device, dtype=torch.long)
+        if kv == "paged":
+            i32 = dict(device=self.device, dtype=torch.int32)
+            gp = torch.Generator().manual_seed(seed)  # any order of pages will do: take a mixed one
+            order = torch.randperm(cache_shape[0], generator=gp).int()
+            tables = torch.full((batch, max(width)), -1, dtype=torch.int32)
+            at = 0
+            for b, n in enumerate(held):
+                tables[b, :n] = order[at:at + n]
+                at += n
+            self.block_tables, self.free_pages = tables.to(self.device), order[at:].to(self.device)
+            self.cached = torch.tensor(lengths, **i32)
+            self.taken = torch.zeros(1, **i32)
+            self._start = (self.cached.clone(), self.taken.clone())
+            self.paged_step: PageSlots | None = None
+        self.top_k = logprobs
+        self.logprobs: TokenLogprobs | None = None
+        self.v_start = self.v_local * self.rank
+        self.v_valid = min(self.v_local, cfg.vocab - self.v_start)
+        if logprobs is not None and not 0 <= logprobs <= min(32, self.v_valid):
+            raise ValueError("logprobs must be from 0 to 32 and at most this rank's share of the vocabulary")
         self._gathered = torch.empty(W * batch * 2, device=self.device, dtype=torch.float32)
 
     # --------------------------------------------------------------- pieces --
@@ -220,10 +271,17 @@ class LlamaTPDecoder:
         cfg, ops = self.cfg, self.ops
         torch.index_select(self.embed, 0, self.tokens, out=self.h)
         self.x.copy_(F.rms_norm(self.h, (cfg.hidden,), self.layers[0]["in_norm"], cfg.eps))
+        if self.kv == "paged":
+            paged = self.paged_step = assign_pages(self.cached, self.block_tables, self.free_pages, self.taken,
+                                                   self.page_size)
         for i, L in enumerate(self.layers):
             self._proj(self.x, self._w(i, "wqkv"), self.qkv)
             attn = self.attn.view(self.B, self.Hq, cfg.head_dim)
-            if self.impl == "baseline":
+            if self.kv == "paged":
+                rope_append_paged(self.qkv, self.cos, self.sin, paged.positions, paged.slots, L["k"], L["v"], self.Hq,
+                                  out=self.q)
+                paged_attention(self.q, L["k"], L["v"], self.block_tables, paged.lengths, out=attn)
+            elif self.impl == "baseline":
                 ops.rope_append(self.qkv, self.cos, self.sin, self.pos, self.q, L["k"], L["v"], self.Hq, self.Hkv)
                 ops.decode_attention(self.q, L["k"], L["v"], self.pos, attn, self.splits)
             elif self.attention == "tc":
@@ -252,6 +310,10 @@ class LlamaTPDecoder:
             self.next_tokens.copy_(allv[best, torch.arange(self.B, device=self.device), 1].long())
         else:
             self.next_tokens.copy_(idx)
+        if self.top_k is not None:
+            # columns past the vocabulary pad the last shard's weight
+            r = token_logprobs(self.logits[:, :self.v_valid], self.next_tokens, self.top_k, self.v_start)
+            self.logprobs = gather_token_logprobs(r) if self.world > 1 else r
         if check_enabled() and not torch.cuda.is_current_stream_capturing():
             check_kernels()
             if self.comm is not None:
@@ -260,6 +322,18 @@ class LlamaTPDecoder:
 
     def reset_position(self):
         self.pos.fill_(self.ctx)
+        if self.kv == "paged":
+            self.cached.copy_(self._start[0])
+            self.taken.copy_(self._start[1])
+
+    def advance(self):
+        """Makes the last step's tokens, lengths and pages the next step's
+        (``kv="paged"``; graph-capturable after :meth:`step`)."""
+        if self.kv != "paged" or self.paged_step is None:
+            raise ValueError("advance needs kv='paged' and a step")
+        self.tokens.copy_(self.next_tokens)
+        self.cached.copy_(self.paged_step.lengths)
+        self.taken.copy_(self.paged_step.taken)
 
     @torch.no_grad()
     def reference_step_fp32(self) -> list[torch.Tensor]:
@@ -270,6 +344,8 @@ class LlamaTPDecoder:
         this function's own (the cache is not written)."""
         if self.world != 1:
             raise ValueError("the fp32 reference runs on one GPU (world size 1 or shard_of)")
+        if self.kv != "contiguous":
+            raise ValueError("the fp32 reference reads a contiguous cache")
         cfg = self.cfg
         D, B, Hq, Hkv = cfg.head_dim, self.B, self.Hq, self.Hkv
         pos = int(self.pos.item())

@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple, Sequence
 
 import torch
+import torch.distributed as dist
 
 from . import _ext
 from .errors import after_launch
@@ -63,3 +64,19 @@ def join_token_logprobs(shards: Sequence[TokenLogprobs]) -> TokenLogprobs:
     order = raw.nan_to_num(nan=-torch.inf, posinf=torch.inf, neginf=-torch.inf)
     order = order.argsort(dim=-1, descending=True, stable=True)[:, :k]
     return TokenLogprobs(logprob, entropy, lse, top.gather(-1, order), ids.gather(-1, order), raw.gather(-1, order))
+
+
+def gather_token_logprobs(shard: TokenLogprobs, group=None) -> TokenLogprobs:
+    """:func:`join_token_logprobs` over the ranks of a process group, each with
+    its shard of the vocabulary in rank order: one all-gather of
+    ``3 + 3 top_k`` floats per row (token ids below 2^24). Every rank gets the
+    whole vocabulary's result."""
+    rows, k = shard.top_logprobs.shape
+    mine = torch.cat([torch.stack([shard.logprob, shard.entropy, shard.lse], -1), shard.top_logprobs,
+                      shard.top_tokens.float(), shard.top_logits], -1)
+    world = dist.get_world_size(group)
+    parts = torch.empty(world * rows, 3 + 3 * k, dtype=mine.dtype, device=mine.device)
+    dist.all_gather_into_tensor(parts, mine.contiguous(), group=group)
+    return join_token_logprobs([
+        TokenLogprobs(p[:, 0], p[:, 1], p[:, 2], p[:, 3:3 + k], p[:, 3 + k:3 + 2 * k].long(), p[:, 3 + 2 * k:])
+        for p in parts.view(world, rows, 3 + 3 * k)])

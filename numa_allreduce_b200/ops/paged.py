@@ -85,9 +85,10 @@ def rope_append_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
     All of it in fp32, rounded once.
 
     k and v of token ``t`` go to slot ``slots[t]``; slots must be distinct,
-    and a token with slot -1 is not stored. A slot past the cache is not
-    stored and a position outside the tables is clamped to them; both are
-    recorded (:func:`~numa_allreduce_b200.check_kernels`). Returns q as
+    and a token with slot -1 is not stored. A token with a slot past the cache
+    is not stored either, and a position outside the tables is clamped to
+    them; both (the latter for tokens with a slot) are recorded
+    (:func:`~numa_allreduce_b200.check_kernels`). Returns q as
     ``[tokens, q_heads, head_dim]``.
     """
     ops = _ext.load()

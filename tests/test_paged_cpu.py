@@ -233,3 +233,46 @@ def test_join_of_shards_is_the_whole_vocabulary(shards):
 def test_join_of_no_shards():
     with pytest.raises(ValueError):
         nab.join_token_logprobs([])
+
+
+def _gather(rank, world, port, path):
+    import torch.distributed as dist
+
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=world)
+    g = torch.Generator().manual_seed(3)
+    x = ((torch.randn(4, 50 * world, generator=g, dtype=torch.float64) * 3) * 4).round() / 4
+    tokens = torch.tensor([0, 49, 50, 99])
+    parts = [_oracle(x[:, 50 * i:50 * (i + 1)], tokens, 5, 50 * i) for i in range(world)]
+    got = nab.gather_token_logprobs(parts[rank])
+    torch.save((got, nab.join_token_logprobs(parts)), f"{path}/{rank}.pt")
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_gather_over_ranks(tmp_path):
+    import torch.multiprocessing as mp
+
+    from conftest import free_port
+
+    mp.spawn(_gather, args=(2, free_port(), str(tmp_path)), nprocs=2)
+    for rank in range(2):
+        got, want = torch.load(tmp_path / f"{rank}.pt", weights_only=False)
+        assert torch.equal(got.top_tokens, want.top_tokens)
+        for a, b in zip(got, want):
+            torch.testing.assert_close(a, b, rtol=0, atol=1e-13)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(kv="pages"), "kv must be"),
+    (dict(lengths=[3]), "needs kv='paged'"),
+    (dict(kv="paged", page_size=24), "page_size"),
+    (dict(kv="paged", page_size=0), "page_size"),
+    (dict(kv="paged", max_new=0), "max_new"),
+    (dict(kv="paged", lengths=[3, 4]), "one length per request"),
+    (dict(kv="paged", lengths=[-1]), "one length per request"),
+])
+def test_decoder_refuses(kw, match):
+    from numa_allreduce_b200.models.llama_tp import LlamaConfig, LlamaTPDecoder
+
+    with pytest.raises(ValueError, match=match):
+        LlamaTPDecoder(LlamaConfig.tiny(), None, batch=1, context=4, device="cpu", **kw)
