@@ -37,7 +37,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, v
     For inference: logits that require a gradient are refused.
     """
     ops = _ext.load()
-    r = TokenLogprobs(*ops.token_logprobs.default(logits, tokens, top_k, vocab_start))
+    r = TokenLogprobs._make(ops.token_logprobs.default(logits, tokens, top_k, vocab_start))
     after_launch()
     return r
 

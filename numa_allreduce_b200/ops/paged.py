@@ -63,8 +63,8 @@ def assign_pages(cached: torch.Tensor, block_tables: torch.Tensor, free_pages: t
         if query_start is not None:
             raise ValueError("assign_pages needs num_tokens with query_start")
         num_tokens = cached.shape[0]
-    r = PageSlots(*ops.assign_pages.default(cached, query_start, block_tables, free_pages, taken, page_size,
-                                            num_tokens))
+    r = PageSlots._make(ops.assign_pages.default(cached, query_start, block_tables, free_pages, taken, page_size,
+                                                 num_tokens))
     after_launch()
     return r
 
