@@ -69,7 +69,7 @@ constexpr int kBoxRows = 16;    // rows of the smallest TMA box, and of one step
 constexpr int kWarps = 4;       // computing warps
 constexpr int kPThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;       // query heads of one head tile (the MMA's M)
-constexpr int kJoinThreads = 256, kFewThreads = 128;
+constexpr int kJoinThreads = 512, kFewThreads = 128;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -98,7 +98,10 @@ struct PagedDev {
   void* out;
   float* ws_o;    // [2 * grid][16][D]: parts
   float2* ws_ml;  // [2 * grid][16]: their (max, sum)
-  int4* desc;     // [grid]: the cut segment that begins in a CTA (output row, heads, last CTA, 1 + inside), or w = 0
+  // (output row, heads, first CTA, last CTA * 2 + inside) of a cut segment, or heads = 0: of the one that begins in
+  // a CTA, or with by_segment of each segment (fewer than CTAs)
+  int4* desc;
+  int by_segment;
   int num_pages;
   int B, M, P, Hq, Hkv;
   int G;          // query heads per kv head
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kPThreads, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(paged_smem + C::kBars);
   uint64_t* empty = full + S;
   uint64_t* q_empty = empty + S;
-  int* misc = reinterpret_cast<int*>(paged_smem + C::kMisc);  // abort, b, first unit of b, -, warp sums
+  int* misc = reinterpret_cast<int*>(paged_smem + C::kMisc);  // abort, b, first unit of b, -, warp sums, warp maxima
   volatile int* abort_flag = misc;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int HH = a.Hkv * a.HT;
@@ -249,29 +252,39 @@ __global__ void __launch_bounds__(kPThreads, 2)
       const int len = length_of(a, b);
       return a.whole ? (len > 0) : (len + kTile - 1) / kTile;
     };
-    int mine = 0;
+    int mine = 0, most = 0;
     for (int b = rb0; b < rb1; ++b) {
       const int raw = a.lengths[b];
       if (blockIdx.x == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
         record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(b));
-      mine += units(b);
+      const int n = units(b);
+      mine += n;
+      most = max(most, n);
     }
+    most = __reduce_max_sync(0xffffffffu, most);
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += y;
     }
-    if (lane == 31) misc[4 + warp] = incl;
+    if (lane == 31) {
+      misc[4 + warp] = incl;
+      misc[4 + kPThreads / 32 + warp] = most;
+    }
     __syncthreads();
     int before = incl - mine, total = 0;
 #pragma unroll
     for (int i = 0; i < kPThreads / 32; ++i) {
       before += i < warp ? misc[4 + i] : 0;
       total += misc[4 + i];
+      most = max(most, misc[4 + kPThreads / 32 + i]);
     }
     const int W = total * HH;
     per = max(1, (W + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    // A tile takes its CTA 0.55 us, a part the join 0.014 us: with p tiles per CTA the longest segment of `most`
+    // tiles costs 0.55 p + 0.014 most / p, least at p = sqrt(most / 39).
+    if (!a.whole) per = max(per, static_cast<int>(ceilf(sqrtf(static_cast<float>(most) * (1.f / 39.f)))));
     const int64_t lo64 = static_cast<int64_t>(blockIdx.x) * per;
     lo = static_cast<int>(min64(lo64, W));
     const int hi = static_cast<int>(min64(lo64 + per, W));
@@ -411,8 +424,10 @@ __global__ void __launch_bounds__(kPThreads, 2)
       if (length_of(a, b) > 0) continue;
       uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.Hq * D);
       for (int i = tid; i < a.Hq * D / 8; i += 32 * kWarps) o[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (a.by_segment)
+        for (int i = tid; i < HH; i += 32 * kWarps) a.desc[b * HH + i] = make_int4(0, 0, 0, 0);
     }
-    if (tid == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0 && !a.whole && !a.by_segment) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
 
   constexpr int kNt = D / 8;           // output column tiles
@@ -663,10 +678,11 @@ __global__ void __launch_bounds__(kPThreads, 2)
             if (t4 == 0) a.ws_ml[part * kRows + row] = make_float2(m[r], l[r]);
           }
         }
-        if (t0 == 0 && lane == 0) {
-          const int last = (w.x + w.nt - 1) / per;  // CTA of the last tile
-          a.desc[blockIdx.x] = make_int4(static_cast<int>(row0), heads, last, 1 + (w.x != lo));
-        }
+      }
+      if (lane == 0 && t0 == 0 && !a.whole && (n < w.nt || a.by_segment)) {
+        const int last = (w.x + w.nt - 1) / per;  // CTA of the last tile
+        a.desc[a.by_segment ? w.b * HH + w.h : blockIdx.x] =
+            make_int4(static_cast<int>(row0), n < w.nt ? heads : 0, blockIdx.x, 2 * last + (w.x != lo));
       }
     }
     ++seg;
@@ -726,12 +742,11 @@ __global__ void __launch_bounds__(kPThreads, 2)
   }
 }
 
-// Joins the parts of the segment that begins in main CTA blockIdx.x, if one
-// that is cut does, in order: o = sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i. Two
+// Joins the parts of cut segment desc[blockIdx.x], in order: o = sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i. Two
 // forms:
 //   few   a thread per 4 dims of a head, the parts one after the other with 8
 //         loads in flight, for many heads and few parts;
-//   many  blockIdx.y takes a head, groups of D / 4 threads every eighth part.
+//   many  blockIdx.y takes a head, groups of D / 4 threads every n-th part.
 // Time that the join adds to the main kernel (us, few / many): 64 requests of
 // up to 8192, 8 heads of 128 dims 4.5 / 6.2; 32 of up to 2500, 16 heads 3.2 /
 // 7.0, 4 heads 3.2 / 3.0; 37 parts of 4 heads of 64 dims 8.3 / 3.4.
@@ -740,11 +755,11 @@ __global__ void __launch_bounds__(kFewThreads) k_paged_join_few(const __grid_con
   constexpr int kAhead = 8;
   pdl_wait();
   pdl_trigger();
-  const int c = blockIdx.x, at = blockIdx.y * kFewThreads + threadIdx.x;
-  const int4 d = a.desc[c];
+  const int at = blockIdx.y * kFewThreads + threadIdx.x;
+  const int4 d = a.desc[blockIdx.x];
   const int row = at / (D / 4), col = at % (D / 4) * 4;
-  if (d.w == 0 || row >= d.y) return;
-  const int count = d.z - c + 1;
+  if (row >= d.y) return;
+  const int c = d.z, count = (d.w >> 1) - c + 1;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, L = 0.f;
   for (int i0 = 0; i0 < count; i0 += kAhead) {
@@ -755,7 +770,7 @@ __global__ void __launch_bounds__(kFewThreads) k_paged_join_few(const __grid_con
       ml[i] = make_float2(-INFINITY, 0.f);
       x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i0 + i < count) {
-        const int64_t part = 2 * static_cast<int64_t>(c + i0 + i) + (i0 + i == 0 ? d.w - 1 : 0);
+        const int64_t part = 2 * static_cast<int64_t>(c + i0 + i) + (i0 + i == 0 ? d.w & 1 : 0);
         ml[i] = a.ws_ml[part * kRows + row];
         x[i] = *reinterpret_cast<const float4*>(a.ws_o + (part * kRows + row) * D + col);
       }
@@ -792,17 +807,15 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
   __shared__ float s_m[kGroups], s_l[kGroups];
   pdl_wait();
   pdl_trigger();
-  const int c = blockIdx.x;
-  const int4 d = a.desc[c];
-  if (d.w == 0) return;
+  const int4 d = a.desc[blockIdx.x];
   const int grp = threadIdx.x / kLanes, ln = threadIdx.x % kLanes;
-  const int pieces = d.z - c + 1;
+  const int c = d.z, pieces = (d.w >> 1) - c + 1;
   for (int row = blockIdx.y; row < d.y; row += gridDim.y) {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
 #pragma unroll 4
     for (int i = grp; i < pieces; i += kGroups) {
-      const int64_t part = 2 * static_cast<int64_t>(c + i) + (i == 0 ? d.w - 1 : 0);
+      const int64_t part = 2 * static_cast<int64_t>(c + i) + (i == 0 ? d.w & 1 : 0);
       const float2 ml = a.ws_ml[part * kRows + row];
       const float4 x = *reinterpret_cast<const float4*>(a.ws_o + (part * kRows + row) * D + 4 * ln);
       const float mn = fmaxf(m, ml.x);
@@ -888,6 +901,7 @@ struct PagedPlan {
   int cluster;   // CTAs per segment in the cluster form, 0 for the others
   bool whole;    // ranges of whole segments
   bool few;      // which form of the join
+  int descs;     // segments that it may have to join
   int box_rows;
 };
 
@@ -913,6 +927,7 @@ PagedPlan plan_of(int B, int M, int P, int Hq, int Hkv, int D, int sms) {
   p.whole = !p.cluster && tiles <= 4;
   p.grid = static_cast<int>(p.cluster ? segments * c : std::min<int64_t>(slots, p.whole ? segments : tiles * segments));
   // parts of a segment when all requests are of one length: grid / segments and two ends
+  p.descs = static_cast<int>(std::min<int64_t>(segments, p.grid));
   p.few = p.grid / segments + 2 <= 8 && p.GT * D >= 4 * kFewThreads;
   p.box_rows = tile;
   while (P % p.box_rows != 0) p.box_rows /= 2;  // P is a multiple of 16
@@ -964,6 +979,7 @@ void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
   a.desc = reinterpret_cast<int4*>(a.ws_ml + static_cast<int64_t>(p.grid) * 2 * kRows);
   a.cluster = p.cluster;
   a.whole = p.whole;
+  a.by_segment = !p.cluster && !p.whole && p.descs < p.grid;
   a.box_rows = p.box_rows;
   a.num_pages = static_cast<int>(in.num_pages);
   a.B = in.B;
@@ -998,9 +1014,9 @@ void run(cudaStream_t s, const PagedAttnArgs& in, int dtype, int sms) {
     void* join_args[1] = {&a};
     if (p.few) {
       launch(reinterpret_cast<const void*>(&k_paged_join_few<T, D>),
-             dim3(p.grid, (p.GT * (D / 4) + kFewThreads - 1) / kFewThreads), kFewThreads, 0, 0, s, join_args);
+             dim3(p.descs, (p.GT * (D / 4) + kFewThreads - 1) / kFewThreads), kFewThreads, 0, 0, s, join_args);
     } else {
-      launch(reinterpret_cast<const void*>(&k_paged_join<T, D>), dim3(p.grid, p.GT), kJoinThreads, 0, 0, s, join_args);
+      launch(reinterpret_cast<const void*>(&k_paged_join<T, D>), dim3(p.descs, p.GT), kJoinThreads, 0, 0, s, join_args);
     }
   }
 }
