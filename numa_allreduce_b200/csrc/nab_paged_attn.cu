@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(kPThreads, 2)
   // row % 8); column step j is 32 bytes on, i.e. XOR j << 5.
   const uint32_t k_off = (warp * kSteps * kBoxRows + lr + (lm >> 1) * 8) * 128 + (((lm & 1) ^ lr) << 4);
   const uint32_t v_off = (warp * kSteps * kBoxRows + lr + (lm & 1) * 8) * 128 + (((lm >> 1) ^ lr) << 4);
-  uint32_t qf[D / 16][4];
+  // Q fragments: per 16-dim step rows 0-7 and 8-15, or (up to 8 heads) of two steps rows 0-7
+  uint32_t qf[kWide ? D / 16 : D / 32][4];
   int tile = 0, seg = 0;
   bool dead = false;
   // a segment's running maximum, sum and output of this warp's positions
@@ -457,17 +458,19 @@ __global__ void __launch_bounds__(kPThreads, 2)
     for (int j = 0; j < 2; ++j) odd[j][0] = odd[j][1] = odd[j][2] = odd[j][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
+      const uint32_t q4[4] = {kWide ? qf[k][0] : qf[k >> 1][2 * (k & 1)], kWide ? qf[k][1] : 0u,
+                              kWide ? qf[k][2] : qf[k >> 1][2 * (k & 1) + 1], kWide ? qf[k][3] : 0u};
 #pragma unroll
       for (int x = 0; x < kSteps; ++x) {
         // matrices: (positions 0-7 | 8-15 by lm >> 1) x (dims 0-7 | 8-15 by lm & 1)
         uint32_t kf[4];
         ldsm4((kb ^ ((k & 3) << 5)) + (k >> 2) * C::kBlock + x * kBoxRows * 128, kf);
         if (kChains == 2 && (k & 1)) {
-          mma16816<T>(odd[0], qf[k], kf[0], kf[1]);
-          mma16816<T>(odd[1], qf[k], kf[2], kf[3]);
+          mma16816<T>(odd[0], q4, kf[0], kf[1]);
+          mma16816<T>(odd[1], q4, kf[2], kf[3]);
         } else {
-          mma16816<T>(sc[2 * x], qf[k], kf[0], kf[1]);
-          mma16816<T>(sc[2 * x + 1], qf[k], kf[2], kf[3]);
+          mma16816<T>(sc[2 * x], q4, kf[0], kf[1]);
+          mma16816<T>(sc[2 * x + 1], q4, kf[2], kf[3]);
         }
       }
     }
@@ -569,12 +572,14 @@ __global__ void __launch_bounds__(kPThreads, 2)
       }
       if (!dead) {
         if (i == 0) {
-          // Q fragments: A rows are heads; matrices (rows 0-7 | 8-15) x (dims 0-7 | 8-15) of each 16-dim step
+          // A rows are heads; matrices, by lm: (rows 0-7 | 8-15) x (dims 0-7 | 8-15) of a step, or (rows 0-7) x
+          // (dims 0-7 | 8-15) of two steps
           const uint32_t qb = base + C::kQ + (seg & 1) * C::kQBytes;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const int row = lr + (lm & 1) * 8, chunk = (k & 3) * 2 + (lm >> 1);
-            ldsm4(qb + (k >> 2) * kQHalf + row * 128 + ((chunk ^ (row & 7)) << 4), qf[k]);
+          for (int k = 0; k < (kWide ? D / 16 : D / 32); ++k) {
+            const int step = kWide ? k : 2 * k + (lm >> 1);
+            const int row = kWide ? lr + (lm & 1) * 8 : lr, chunk = (step & 3) * 2 + (kWide ? lm >> 1 : lm & 1);
+            ldsm4(qb + (step >> 2) * kQHalf + row * 128 + ((chunk ^ lr) << 4), qf[k]);
           }
           __syncwarp();
           if (lane == 0) sm100::mbar_arrive(&q_empty[seg & 1]);
