@@ -239,10 +239,12 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   const int p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);  // this CTA's pieces
   const int i0 = max(p0, r.mis > 0), i1 = min(p1, (r.mis + a.V) / N);  // those within the row
   const int k = a.top_k;
-  float picked = -INFINITY;  // the given token's logit
+  float picked = 0.f;  // the given token's logit, if it is in this part of the vocabulary
+  bool here = false;
   if (tid == 0 && part == 0) {
-    const int64_t at = a.tokens[row] - a.vocab_start;
-    if (at >= 0 && at < a.V) picked = static_cast<float>(r.x[at]);
+    const int64_t token = a.tokens[row];  // any value
+    here = token >= a.vocab_start && token - a.vocab_start < a.V;
+    if (here) picked = static_cast<float>(r.x[token - a.vocab_start]);
   }
 
   // ------------------------------------------------------- one pass --
@@ -510,8 +512,6 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       return x < kFloor ? x - lse : (fmaf(x, kL2e, -scaled) - log2_s) * kLn2;
     };
     if (tid == 0) {
-      const int64_t at = a.tokens[row] - a.vocab_start;
-      const bool here = at >= 0 && at < a.V;
       a.logprob[row] = here ? logprob_of(picked) : -INFINITY;
       a.lse[row] = lse;
       a.entropy[row] = (log2_s - all.u / all.s) * kLn2;

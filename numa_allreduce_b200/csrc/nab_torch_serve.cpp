@@ -119,22 +119,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1) &&
                   (B == 1 || block_tables.stride(0) >= block_tables.size(1)),
               op, ": block_tables must be int32 [", B, ", pages], each row contiguous and apart from the others");
-  TORCH_CHECK(block_tables.size(1) * B < INT_MAX, op, ": block_tables is too large");
+  // the kernel's indices run a grid's width past these
+  TORCH_CHECK(block_tables.size(1) * B <= (1 << 30), op, ": block_tables is too large");
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.is_contiguous() && free_pages.scalar_type() == at::kInt &&
                   free_pages.size(0) < INT_MAX,
               op, ": free_pages must be a contiguous int32 vector");
   check_vector(op, "taken", taken, at::kInt, 1);
   TORCH_CHECK(page_size >= 16 && page_size % 16 == 0 && page_size <= (1 << 20), op,
               ": page_size must be a multiple of 16, got ", page_size);
-  TORCH_CHECK(num_tokens >= 0 && num_tokens < INT_MAX, op, ": bad num_tokens ", num_tokens);
+  TORCH_CHECK(num_tokens >= 0 && num_tokens <= (1 << 30), op, ": bad num_tokens ", num_tokens);
   TORCH_CHECK(query_start || num_tokens >= B, op, ": num_tokens must be at least the ", B, " requests");
   check_devices(op, {{"cached", &cached},
                      {"query_start", query_start ? &*query_start : nullptr},
                      {"block_tables", &block_tables},
                      {"free_pages", &free_pages},
                      {"taken", &taken}});
-  at::assert_no_overlap(block_tables, cached);
-  at::assert_no_overlap(block_tables, free_pages);
+  for (const at::Tensor* t : {&cached, &free_pages, &taken}) at::assert_no_overlap(block_tables, *t);
+  if (query_start) at::assert_no_overlap(block_tables, *query_start);
   const at::cuda::CUDAGuard guard(cached.device());
   Outputs outputs(cached);
   outputs.add({num_tokens}, at::kInt);
@@ -205,6 +206,10 @@ at::Tensor rope_append_paged_to(const at::Tensor& qkv, const at::Tensor& cos, co
                      {"q_norm", q_norm ? &*q_norm : nullptr},
                      {"k_norm", k_norm ? &*k_norm : nullptr},
                      {"out", given}});
+  for (const at::Tensor* t : {&k_pages, &v_pages}) {
+    at::assert_no_overlap(*t, qkv);
+    if (given) at::assert_no_overlap(*given, *t);
+  }
   if (given) at::assert_no_overlap(*given, qkv);
   const at::cuda::CUDAGuard guard(qkv.device());
   at::Tensor out = given ? *given : fresh({T, Hq, D}, qkv.scalar_type(), qkv);
@@ -276,7 +281,9 @@ at::Tensor paged_attention_to(const at::Tensor& q, const at::Tensor& k_pages, co
                      {"block_tables", &block_tables},
                      {"lengths", &lengths},
                      {"out", given}});
-  if (given) at::assert_no_overlap(*given, q);
+  if (given) {
+    for (const at::Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(*given, *t);
+  }
   const at::cuda::CUDAGuard guard(q.device());
   at::Tensor out = given ? *given : fresh({B, Hq, D}, q.scalar_type(), q);
   if (B == 0) return out;

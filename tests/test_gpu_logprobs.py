@@ -88,6 +88,9 @@ def test_tokens_outside_the_vocabulary():
     t = torch.tensor([-1, -100, 50, 2 ** 62], device="cuda")
     r = check(logits(4, 50, F32, 5), t, 3)
     assert (r.logprob == -math.inf).all()
+    far = torch.tensor([-2 ** 63, 2 ** 63 - 1, 6, 7], device="cuda")
+    r = nab.token_logprobs(logits(4, 50, F32, 5), far, vocab_start=7)
+    assert (r.logprob[:3] == -math.inf).all() and torch.isfinite(r.logprob[3])
 
 
 @pytest.mark.parametrize("v", [50, 4096, 40000])

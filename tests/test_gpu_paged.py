@@ -342,12 +342,17 @@ def test_paged_attention(lengths, hq, hkv, d, page, dtype):
     nab.check_kernels()
 
 
-@pytest.mark.parametrize("batch,most,hq,hkv,page", [(161, 40, 8, 1, 16), (700, 90, 8, 8, 32), (64, 3000, 8, 2, 64),
-                                                    (5, 9000, 64, 8, 16)])
+@pytest.mark.parametrize("batch,most,hq,hkv,page", [
+    (161, 40, 8, 1, 16), (700, 90, 8, 8, 32), (64, 3000, 8, 2, 64), (5, 9000, 64, 8, 16),
+    (50, 1500, 64, 8, 64), (50, 1500, 16, 8, 48),   # more segments than CTAs, cut ones among them
+    (100, 300, 4, 1, 16), (40, 500, 8, 1, 32), (9, 1100, 12, 1, 64),  # clusters of 2, 4 and 8
+    (290, 70, 8, 1, 128), (400, 250, 3, 1, 16),
+])
 def test_paged_attention_ragged_batches(batch, most, hq, hkv, page):
-    """More requests than threads, ranges that begin and end inside requests."""
+    """More requests than threads, ranges that begin and end inside requests, requests without positions."""
     g = torch.Generator().manual_seed(batch)
     lengths = torch.randint(0, most + 1, (batch,), generator=g).tolist()
+    lengths[batch // 2] = 0
     k, v, tables = make_cache(lengths, hkv, 128, page, BF, seed=batch)
     q = torch.randn(batch, hq, 128, generator=gen(2), device="cuda").to(BF)
     out = nab.paged_attention(q, k, v, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
@@ -419,6 +424,21 @@ def test_paged_attention_records_bad_lengths_and_pages():
         k2, v2 = (torch.cat([x, torch.zeros_like(x[:1])]) for x in (k, v))
         t[0, 1] = k.shape[0]
         check_attention(out, q, k2, v2, t, [64, 64], 128 ** -0.5)
+
+
+def test_overlapping_tensors_are_refused():
+    pool = torch.zeros(3, 1, 16, 64, device="cuda", dtype=BF)
+    cos, sin = nab.rope_tables(4, 64)
+    i = torch.zeros(1, device="cuda", dtype=torch.int32)
+    q = torch.zeros(1, 2, 64, device="cuda", dtype=BF)
+    with pytest.raises(RuntimeError, match="overlap|single memory"):
+        nab.paged_attention(q, pool[:2], pool[1:], i[None], i)
+    with pytest.raises(RuntimeError, match="overlap|single memory"):
+        nab.paged_attention(q, pool, pool.clone(), i[None], i, out=q)
+    with pytest.raises(RuntimeError, match="overlap|single memory"):
+        nab.rope_append_paged(pool.view(-1)[:256].view(1, 256), cos, sin, i, i.long(), pool, pool.clone(), 2)
+    with pytest.raises(RuntimeError, match="overlap|single memory"):
+        nab.assign_pages(i, i[None], i, i.clone(), 16)
 
 
 def test_paged_attention_empty_calls():
