@@ -41,15 +41,19 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const __grid_co
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int taken = *a.taken;  // in flight during the scan
   auto new_tokens = [&](int b) { return a.starts ? max(0, a.starts[b + 1] - a.starts[b]) : 1; };
-  auto pages_of = [&](int64_t n) { return static_cast<int>(min64((n + a.P - 1) / a.P, a.M)); };
+  auto pages_of = [&](uint32_t n) {  // n up to 2^31 + 2^30
+    const uint32_t P = a.P;
+    return static_cast<int>(min(n / P + (n % P != 0), static_cast<uint32_t>(a.M)));
+  };
   int total = 0;
   for (int b0 = 0; b0 < a.B; b0 += kAssignThreads) {
     const int b = b0 + tid;
     int need = 0;
     if (b < a.B) {
       const int c = max(0, a.cached[b]);
-      need = pages_of(static_cast<int64_t>(c) + new_tokens(b)) - pages_of(c);
+      need = pages_of(static_cast<uint32_t>(c) + new_tokens(b)) - pages_of(c);
       if (a.starts) start[b] = a.starts[b];
     }
     int x = need;
@@ -72,7 +76,7 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const __grid_co
   }
   if (a.starts && tid == 0) start[a.B] = a.starts[a.B];
   __syncthreads();
-  const int used = min(max(0, *a.taken), a.F);
+  const int used = min(max(0, taken), a.F);
   const int avail = a.F - used;
   const int gtid = blockIdx.x * kAssignThreads + tid, gsize = gridDim.x * kAssignThreads;
 
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const __grid_co
   }
   for (int b = gtid; b < a.B; b += gsize) {
     const int c = max(0, a.cached[b]), old = pages_of(c);
-    const int64_t end = static_cast<int64_t>(c) + new_tokens(b);
+    const uint32_t end = static_cast<uint32_t>(c) + new_tokens(b);
     const int have = old + min(max(0, avail - off[b]), pages_of(end) - old);
     a.lengths[b] = static_cast<int>(min64(min64(end, static_cast<int64_t>(have) * a.P), 0x7fffffff));
   }
@@ -107,21 +111,22 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const __grid_co
       live = t >= start[b] && t < start[b + 1];
       row = t - start[b];
     }
-    int64_t pos = 0, slot = -1;
+    uint32_t pos = 0;  // up to 2^31 + 2^30
+    int64_t slot = -1;
     if (live) {
       const int c = max(0, a.cached[b]), old = pages_of(c);
-      pos = static_cast<int64_t>(c) + row;
-      const int64_t j = pos / a.P;
+      pos = static_cast<uint32_t>(c) + row;
+      const int j = static_cast<int>(pos / static_cast<uint32_t>(a.P));
       int page = -1;
       if (j < old) {
         page = a.tables[b * a.table_stride + j];
       } else if (j < a.M) {
-        const int i = off[b] + static_cast<int>(j - old);
+        const int i = off[b] + (j - old);
         if (i < avail) page = a.free_pages[used + i];
       }
-      if (page >= 0) slot = static_cast<int64_t>(page) * a.P + (pos - j * a.P);
+      if (page >= 0) slot = static_cast<int64_t>(page) * a.P + (pos - static_cast<uint32_t>(j) * a.P);
     }
-    a.positions[t] = static_cast<int>(min64(pos, 0x7fffffff));
+    a.positions[t] = static_cast<int>(min(pos, 0x7fffffffu));
     a.slots[t] = slot;
   }
 }

@@ -117,6 +117,7 @@ def run_assign(cached, new, page, width, n_free, taken, pad, seed, row_gap=0):
     # the table is too narrow
     ([30, 40, 100], [10, 30, 4], 16, 3, 20, 0, 1),
     ([16, 48], [40, 1], 48, 2, 5, 0, 0),
+    ([2 ** 31 - 1, 5, 2 ** 31 - 2], None, 16, 3, 4, 0, 1),
 ])
 def test_assign_pages(cached, new, page, width, n_free, taken, pad):
     run_assign(cached, new, page, width, n_free, taken, pad, seed=1)
