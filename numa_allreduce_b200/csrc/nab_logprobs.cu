@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <stdexcept>
 #include <string>
 
@@ -43,6 +44,7 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 1024;  // collected elements of a CTA
 constexpr int kSub = 8;      // parts of a thread's share
+constexpr int kPad = 24 * 1024;  // beside the static 35 KB: three CTAs per SM
 constexpr int kCoarse = 64;  // parts that give the cut: the threads of one remainder mod 64
 constexpr float kL2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -102,12 +104,24 @@ NAB_DINLINE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // How a piece of 16 bytes is read: its kN elements as pairs of floats, its
 // largest element (NaN left out), a word of -inf, and how many of the lowest
 // bits of `ordered` are the same for every value of the type and sign.
+// kFloor: elements below it (masks of any kind, -inf) are raised to it
+// (`raised`, in pairs for 16-bit types; NaN stays) and so count as
+// probability 0 next to any maximum above kLow. Between kLow and kHigh the
+// rounding of log2(e) max is below 2 in the exponent; a row whose maximum lies
+// outside is summed again in another form.
 template <typename T>
 struct Piece;
 template <>
 struct Piece<float> {
   static constexpr uint32_t kFill = 0xff800000u;
   static constexpr int kDrop = 0;
+  static constexpr float kFloor = -0x1p24f, kLow = -0x1p23f, kHigh = 0x1p24f;
+  NAB_DINLINE static uint4 raised(uint4 w) {
+    return make_uint4(__float_as_uint(max_nan(__uint_as_float(w.x), kFloor)),
+                      __float_as_uint(max_nan(__uint_as_float(w.y), kFloor)),
+                      __float_as_uint(max_nan(__uint_as_float(w.z), kFloor)),
+                      __float_as_uint(max_nan(__uint_as_float(w.w), kFloor)));
+  }
   NAB_DINLINE static float largest(uint4 w) {
     return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
@@ -120,6 +134,14 @@ template <>
 struct Piece<__nv_bfloat16> {
   static constexpr uint32_t kFill = 0xff80ff80u;
   static constexpr int kDrop = 16;
+  static constexpr float kFloor = -0x1p24f, kLow = -0x1p23f, kHigh = 0x1p24f;
+  NAB_DINLINE static uint4 raised(uint4 w) {
+    const __nv_bfloat162 f = __floats2bfloat162_rn(kFloor, kFloor);
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+    return w;
+  }
   NAB_DINLINE static float largest(uint4 w) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -136,6 +158,14 @@ template <>
 struct Piece<__half> {
   static constexpr uint32_t kFill = 0xfc00fc00u;
   static constexpr int kDrop = 13;
+  static constexpr float kFloor = -60000.f, kLow = -50000.f, kHigh = 65504.f;
+  NAB_DINLINE static uint4 raised(uint4 w) {
+    const __half2 f = __floats2half2_rn(kFloor, kFloor);
+    __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+    return w;
+  }
   NAB_DINLINE static float largest(uint4 w) {
     const __half2* h = reinterpret_cast<const __half2*>(&w);
     const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
@@ -157,14 +187,15 @@ struct Piece<__half> {
 struct Stats {
   float m, s, u;
 };
-// Values below kFloor count as probability 0 and those above kCeil overflow:
-// a row whose maximum lies out there is summed again in another form.
-constexpr float kFloor = -1e38f, kCeil = 2e38f;
 // (a rounded product of its own: fused into a difference, equal maxima would not cancel)
-NAB_DINLINE float scaled_max(float m) { return __fmul_rn(fmaxf(m, kFloor), kL2e); }
+template <typename T>
+NAB_DINLINE float scaled_max(float m) {
+  return __fmul_rn(fmaxf(m, Piece<T>::kFloor), kL2e);
+}
 // exponents below -1000 count as -1000 (exp2 of them is zero), which keeps 0 * inf out
+template <typename T>
 NAB_DINLINE void raise(Stats& a, float m) {
-  const float d = fmaxf(scaled_max(a.m) - scaled_max(m), -1000.f), f = lp_ex2(d);
+  const float d = fmaxf(scaled_max<T>(a.m) - scaled_max<T>(m), -1000.f), f = lp_ex2(d);
   a.u = f * (a.u + d * a.s);
   a.s *= f;
   a.m = m;
@@ -221,7 +252,7 @@ struct Row {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster) {
+__global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster) {
   __shared__ LpShared sh;
   constexpr int N = Row<T>::kN;
   constexpr int kBatch = 4;
@@ -261,7 +292,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   float big = -INFINITY;  // largest value so far, first held by piece big_at
   float kv = -INFINITY;   // the same within this part
   uint64_t s2 = 0, u2 = 0;
-  float l = scaled_max(big);
+  float l = scaled_max<T>(big);
   const uint64_t l2e = pair(kL2e, kL2e);
   const uint4 fill = make_uint4(Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill, Piece<T>::kFill);
   const uint4* at = reinterpret_cast<const uint4*>(r.x - r.mis) + p0 + tid;  // aligned; piece 0 may begin before x
@@ -300,14 +331,14 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       uint64_t v[N / 2];
-      Piece<T>::pairs(cur[b], v);
+      Piece<T>::pairs(Piece<T>::raised(cur[b]), v);
 #pragma unroll
       for (int e = 0; e < N / 2; ++e) {
-        const float2 d = unpair(fma2(v[e], l2e, neg));
-        const float d0 = max_nan(d.x, -1000.f), d1 = max_nan(d.y, -1000.f);
-        const uint64_t w = pair(lp_ex2(d0), lp_ex2(d1));
+        const uint64_t x = fma2(v[e], l2e, neg);
+        const float2 d = unpair(x);
+        const uint64_t w = pair(lp_ex2(d.x), lp_ex2(d.y));
         s2 = add2(s2, w);
-        u2 = fma2(pair(d0, d1), w, u2);
+        u2 = fma2(x, w, u2);
       }
     }
 #pragma unroll
@@ -339,8 +370,8 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       if (x > part_max.x || (x == part_max.x && q < __float_as_int(part_max.y)))
         part_max = make_float2(x, __int_as_float(q));
       if (x > st.m || (x == st.m && q < big_at)) big_at = q;
-      if (x > st.m) raise(st, x);
-      const float d = max_nan(fmaf(x, kL2e, -scaled_max(st.m)), -1000.f), w = lp_ex2(d);
+      if (x > st.m) raise<T>(st, x);
+      const float d = fmaf(max_nan(x, Piece<T>::kFloor), kL2e, -scaled_max<T>(st.m)), w = lp_ex2(d);
       st.s += w;
       st.u += d * w;
     }
@@ -373,7 +404,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
   top = sh.warp_m[lane % kLpWarps];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  raise(st, top);
+  raise<T>(st, top);
   const float2 sums = block_sum(make_float2(st.s, st.u), sh.warp_s, sh.warp_u);
   if (tid == 0) sh.stats = {top, sums.x, sums.y};
 
@@ -483,7 +514,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       all.s = all.u = 0.f;
 #pragma unroll
       for (int c = 0; c < kMaxCluster; ++c) {
-        raise(part_[c], all.m);
+        raise<T>(part_[c], all.m);
         all.s += c < cluster ? part_[c].s : 0.f;
         all.u += c < cluster ? part_[c].u : 0.f;
       }
@@ -491,9 +522,9 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
     } else if (tid < k) {
       mine = sh.top[tid];
     }
-    // a row whose largest finite value is out of reach of the scaled form: this CTA sums it again as it stands
-    const bool far = all.m > kCeil || all.m < kFloor;
-    if (far && fabsf(all.m) != INFINITY) {
+    const bool far = all.m > Piece<T>::kHigh || all.m < Piece<T>::kLow;
+    if (all.m == -INFINITY && all.s == all.s) all.s = all.u = 0.f;  // nothing but -inf
+    if (far && fabsf(all.m) != INFINITY) {  // this CTA sums the row again as it stands
       float2 sum = make_float2(0.f, 0.f);
       for (int i = tid; i < a.V; i += kLpThreads) {
         const float d = max_nan((static_cast<float>(r.x[i]) - all.m) * kL2e, -1000.f), w = lp_ex2(d);
@@ -505,11 +536,11 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(const __grid_cons
       all.s = sum.x;
       all.u = sum.y;
     }
-    const float log2_s = log2f(all.s), scaled = scaled_max(all.m);
+    const float log2_s = log2f(all.s), scaled = scaled_max<T>(all.m);
     const float lse = far ? all.m + log2_s * kLn2 : (scaled + log2_s) * kLn2;
     auto logprob_of = [&](float x) {
       if (far) return (x - all.m) - log2_s * kLn2;
-      return x < kFloor ? x - lse : (fmaf(x, kL2e, -scaled) - log2_s) * kLn2;
+      return x < Piece<T>::kFloor ? x - lse : (fmaf(x, kL2e, -scaled) - log2_s) * kLn2;
     };
     if (tid == 0) {
       a.logprob[row] = here ? logprob_of(picked) : -INFINITY;
@@ -537,8 +568,8 @@ template <typename T>
 void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
   // CTAs per row. A cluster pays for its two barriers and its slower launch, so only rows of many bytes and few
   // of them are shared: at least 30 KB of logits per CTA, at most two CTAs per SM. Measured with 1 / 2 / 4 / 8
-  // CTAs per row (us, k = 20): 1 x 128256 bf16 12.2 / 10.1 / 8.1 / 7.7; 64 rows 18.0 / 13.7 / 11.6 / 16.1; 148 rows
-  // 18.7 / 16.1 / 18.7 / 26.5; 300 rows 26.0 / 26.6 / 31.7 / 49.0; 1 x 16032 5.4 / 5.9 / 6.1 / 6.9.
+  // CTAs per row (us, k = 20): 1 x 128256 bf16 11.4 / 9.4 / 7.7 / 7.5; 64 rows 15.9 / 12.5 / 11.2 / 13.5; 148 rows
+  // 16.6 / 14.8 / 21.5 / 28.5; 200 rows 18.7 / 21.1 / 24.9 / 34.3; 1 x 16032 5.1 / 5.6 / 5.9 / 6.6.
   int cluster = 1;
   const int64_t bytes = static_cast<int64_t>(a.V) * sizeof(T);
   while (cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * sms && bytes / (cluster * 2) >= 30 * 1024) cluster *= 2;
@@ -548,6 +579,16 @@ void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kLpThreads);
   cfg.stream = s;
+  // Four CTAs fit on an SM; of a grid that fills two to three per SM some SMs would get four and others two. Shared
+  // memory that nobody uses makes it three: 300 x 128256 bf16 30.7 -> 25.2 us.
+  if (grid > 2 * sms && grid <= 3 * sms) cfg.dynamicSmemBytes = kPad;
+  static std::atomic<bool> ready[64];  // by device; setting it twice does no harm
+  int dev = 0;
+  NAB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (cfg.dynamicSmemBytes > 0 && !ready[dev & 63].load(std::memory_order_acquire)) {
+    NAB_CUDA_CHECK(cudaFuncSetAttribute(k_token_logprobs<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPad));
+    ready[dev & 63].store(true, std::memory_order_release);
+  }
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;

@@ -139,8 +139,42 @@ def test_masked_entries(dtype):
     assert r.top_tokens[2].tolist() == [4321] + list(range(19))
 
 
-def test_rows_without_a_distribution():
-    x = logits(5, 5000, F32, 8)
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("mask", [-1e3, -3e4, -1e9, -1e20, -1e30, -3e38])
+def test_finite_masks(mask, dtype):
+    """All but one or a few tokens, or all of them, at a finite value far below."""
+    if dtype == FP and mask < -6e4:
+        mask = -6.5e4
+    for v in (3000, 40000):
+        x = torch.full((4, v), mask, device="cuda", dtype=dtype)
+        x[0, v - 5] = 1.0
+        x[1, 10:14] = torch.tensor([0.5, 2.0, -3.0, 2.0], device="cuda", dtype=dtype)
+        x[2] = -math.inf
+        x[2, ::2] = mask
+        check(x, torch.tensor([v - 5, 12, 4, 100], device="cuda"), 20)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [1e3, 1e6, 1e7, 3e7, 1e12, 1e30])
+def test_large_logits(scale, dtype):
+    check(logits(5, 20000, dtype, 14, scale), tokens(5, 20000), 10)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("v", [5000, 70000])
+def test_rows_near_the_ends_of_the_type(v, dtype):
+    """Maxima around the values where the sums change form, with masked entries beside them."""
+    top = torch.finfo(dtype).max
+    x = logits(10, v, dtype, 13)
+    for i, m in enumerate((-0.97, -0.7, -0.45, -0.2, -0.13, -0.1, 0.1, 0.2, 0.4, 0.97)):
+        x[i] = torch.finfo(dtype).min if i % 2 else -math.inf
+        x[i, 7::3] = top * m
+    check(x, tokens(10, v), 20)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_rows_without_a_distribution(dtype):
+    x = logits(5, 5000, dtype, 8)
     x[0] = -math.inf
     x[1, 77] = math.nan
     x[2, 78] = math.inf
