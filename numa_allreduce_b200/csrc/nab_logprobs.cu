@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   // ------------------------------------------------------- one pass --
   // Piece p is thread (p - p0) % kLpThreads's. Batches of kBatch pieces, the
   // next one's loads in flight during one's arithmetic; pieces past the end
-  // read as -inf, which adds exactly nothing.
+  // read as -inf, i.e. as elements of probability 0.
   const int batches = ((p1 - p0 + kLpThreads - 1) / kLpThreads + kBatch - 1) / kBatch;
   const int sub_batches = max(1, (batches + kSub - 1) / kSub);
   // (value, piece within the CTA), larger = earlier, in as few bits as it takes

@@ -24,7 +24,7 @@
 //            a second launch joins the parts in order. (Joining in the CTA
 //            that finds all parts written needs no second launch but takes
 //            longer: two fences, a read of the flags and the join, 3 to 5 us
-//            that hold up the CTA's next segment, against 2.3 us.)
+//            that hold up the CTA's next segment, against 2.7 to 4 us.)
 //   whole    the same with ranges of whole segments, for short requests: no
 //            part, no second launch.
 //   cluster  calls bound by latency: a thread-block cluster of 1 to 8 CTAs
@@ -600,44 +600,48 @@ __global__ void __launch_bounds__(kPThreads, 2)
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    // warps 2, 3 hand their part to warps 0, 1, then 1 to 0; 8 rows at a time
+    // Warps 2, 3 hand their part to warps 0, 1, then 1 to 0; 8 rows at a time. A short piece has not given all of
+    // them rows.
+    const int active = n > 1 ? kWarps : min(kWarps, (w.len - t0 * kTile + kSteps * kBoxRows - 1) / (kSteps * kBoxRows));
+    auto give = [&](int r, int buffer) {
+      float* mo = reinterpret_cast<float*>(paged_smem + C::kMerge) + buffer * 8 * D;
+      float* ml = reinterpret_cast<float*>(paged_smem + C::kMl) + buffer * 16;
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
+      for (int j = 0; j < kNt; ++j)
+        *reinterpret_cast<float2*>(mo + (j * 8 + g) * 8 + 2 * t4) = make_float2(acc[j][2 * r], acc[j][2 * r + 1]);
+      if (t4 == 0) {
+        ml[2 * g] = m[r];
+        ml[2 * g + 1] = l[r];
+      }
+    };
+    auto take = [&](int r, int buffer) {
+      const float* mo = reinterpret_cast<const float*>(paged_smem + C::kMerge) + buffer * 8 * D;
+      const float* ml = reinterpret_cast<const float*>(paged_smem + C::kMl) + buffer * 16;
+      const float m1 = ml[2 * g], l1 = ml[2 * g + 1];
+      const float mn = fmaxf(m[r], m1);
+      const float ms = mn == -INFINITY ? 0.f : mn;
+      const float w0 = ex2(m[r] - ms), w1 = ex2(m1 - ms);
+      m[r] = mn;
+      l[r] = l[r] * w0 + l1 * w1;
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        float* mo = reinterpret_cast<float*>(paged_smem + C::kMerge) + (warp & 1) * 8 * D;
-        float* ml = reinterpret_cast<float*>(paged_smem + C::kMl) + (warp & 1) * 16;
-        const bool gives = step == 0 ? warp >= 2 : warp == 1;
-        const bool takes = step == 0 ? warp < 2 : warp == 0;
-        if (step == 1 && warp == 0) {
-          mo += 8 * D;
-          ml += 16;
+      for (int j = 0; j < kNt; ++j) {
+        const float2 o = *reinterpret_cast<const float2*>(mo + (j * 8 + g) * 8 + 2 * t4);
+        acc[j][2 * r] = acc[j][2 * r] * w0 + o.x * w1;
+        acc[j][2 * r + 1] = acc[j][2 * r + 1] * w0 + o.y * w1;
+      }
+    };
+    if (active > 1) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        bar_compute();  // the buffers have been read
+        if (active > 2) {
+          if (warp >= 2) give(r, warp & 1);
+          bar_compute();
+          if (warp < 2) take(r, warp);
         }
-        if (gives) {
-#pragma unroll
-          for (int j = 0; j < kNt; ++j)
-            *reinterpret_cast<float2*>(mo + (j * 8 + g) * 8 + 2 * t4) = make_float2(acc[j][2 * r], acc[j][2 * r + 1]);
-          if (t4 == 0) {
-            ml[2 * g] = m[r];
-            ml[2 * g + 1] = l[r];
-          }
-        }
+        if (warp == 1) give(r, 1);
         bar_compute();
-        if (takes) {
-          const float mo_ = ml[2 * g], lo_ = ml[2 * g + 1];
-          const float mn = fmaxf(m[r], mo_);
-          const float ms = mn == -INFINITY ? 0.f : mn;
-          const float w0 = ex2(m[r] - ms), w1 = ex2(mo_ - ms);
-          m[r] = mn;
-          l[r] = l[r] * w0 + lo_ * w1;
-#pragma unroll
-          for (int j = 0; j < kNt; ++j) {
-            const float2 o = *reinterpret_cast<const float2*>(mo + (j * 8 + g) * 8 + 2 * t4);
-            acc[j][2 * r] = acc[j][2 * r] * w0 + o.x * w1;
-            acc[j][2 * r + 1] = acc[j][2 * r + 1] * w0 + o.y * w1;
-          }
-        }
-        if (step == 1) bar_compute();  // the buffers are free again
+        if (warp == 0) take(r, 1);
       }
     }
     const int h0 = (w.h % a.HT) * a.GT;  // first head of the tile within the group
@@ -753,8 +757,9 @@ __global__ void __launch_bounds__(kPThreads, 2)
 //         loads in flight, for many heads and few parts;
 //   many  blockIdx.y takes a head, groups of D / 4 threads every n-th part.
 // Time that the join adds to the main kernel (us, few / many): 64 requests of
-// up to 8192, 8 heads of 128 dims 4.5 / 6.2; 32 of up to 2500, 16 heads 3.2 /
-// 7.0, 4 heads 3.2 / 3.0; 37 parts of 4 heads of 64 dims 8.3 / 3.4.
+// up to 8192, 8 heads of 128 dims 4.0 / 15.6; 32 of up to 2500, 16 heads 2.7 /
+// 16, 4 heads 2.9 / 5.6; 37 parts of 4 heads of 64 dims 7.5 / 3.2; 86 parts of
+// 8 heads of 128 dims 10.4 / 2.9.
 template <typename T, int D>
 __global__ void __launch_bounds__(kFewThreads) k_paged_join_few(const __grid_constant__ PagedDev a) {
   constexpr int kAhead = 8;
@@ -922,13 +927,14 @@ PagedPlan plan_of(int B, int M, int P, int Hq, int Hkv, int D, int sms) {
     throw std::invalid_argument("paged_attention: too many positions for one call");
   // The cluster form takes ceil(tiles / c) tiles one after the other, the even one ceil(tiles * segments / slots) and
   // about three more for its second launch. Measured (us, cluster / even; 8 heads per kv head, D = 128): 1 request of
-  // 1025 6.8 / 6.8, of 4096 11.1 / 7.5; 32 of 2500 12.3 / 15.0; 128 of 1025 17.1 / 20.2. The bound of 10 tiles keeps
-  // ragged batches, where the longest request decides, from losing more than that.
+  // 1025 6.2 / 7.0, of 4096 9.9 / 7.5; 32 of 2500 12.1 / 13.8, of 1 to 2500 9.6 / 11.6; 128 of 1025 16.6 / 18.6. The
+  // bound of 10 tiles keeps ragged batches, where the longest request decides, from losing more than that.
   int c = 1;
   while (c < kMaxCluster && 2 * c <= tiles && segments * c * 2 <= slots) c *= 2;
   const int64_t share = (tiles + c - 1) / c, even = (tiles * segments + slots - 1) / slots;
   p.cluster = segments * c <= slots && share <= std::min<int64_t>(10, even + 3) ? c : 0;
-  // Short requests are not worth a cut: up to 4 tiles of imbalance against the second launch.
+  // Short requests are not worth a cut: up to 4 tiles of imbalance against the second launch (whole / even: 640 of up
+  // to 256 positions 15.9 / 17.0 us, 160 of up to 5 with 4 kv heads 7.7 / 8.7).
   p.whole = !p.cluster && tiles <= 4;
   p.grid = static_cast<int>(p.cluster ? segments * c : std::min<int64_t>(slots, p.whole ? segments : tiles * segments));
   // parts of a segment when all requests are of one length: grid / segments and two ends
