@@ -427,6 +427,17 @@ def test_paged_attention_records_bad_lengths_and_pages():
         check_attention(out, q, k2, v2, t, [64, 64], 128 ** -0.5)
 
 
+def test_checks_after_every_launch_on_request(monkeypatch):
+    monkeypatch.setenv("NAB_CHECK", "1")
+    k, v, tables = make_cache([40], 1, 64, 16, BF, seed=9)
+    q = torch.zeros(1, 2, 64, device="cuda", dtype=BF)
+    n = torch.tensor([40], dtype=torch.int32, device="cuda")
+    nab.paged_attention(q, k, v, tables, n)
+    tables[0, 1] = 10 ** 6
+    with pytest.raises(nab.KernelError, match="out of range"):
+        nab.paged_attention(q, k, v, tables, n)
+
+
 def test_overlapping_tensors_are_refused():
     pool = torch.zeros(3, 1, 16, 64, device="cuda", dtype=BF)
     cos, sin = nab.rope_tables(4, 64)
