@@ -1,16 +1,28 @@
-// Torch bindings of the paged-cache decode operators and the token
-// log-probabilities. They are registered for every backend, so that a bad
-// argument is refused with its name whatever device it lies on; tensors on a
-// device other than CUDA are refused last, and so is one that requires a
-// gradient.
+// Python bindings of the paged-cache decode operators and the token
+// log-probabilities: functions of the extension module itself (PyInit__C),
+// not torch.ops. An eager decode step calls them once or twice per layer, on few
+// tokens, and is bound by the host then: the dispatcher's parsing and boxing of 4 to 13
+// arguments took 2.4 us of a call of 8.8 (8 tokens: pages 8.8 -> 5.9 us, append
+// 8.3 -> 4.6, attention 8.5 -> 5.2, log-probabilities 8.9 -> 6.1, with the check below
+// in place of a look into os.environ, 0.6 us).
+//
+// Every argument is checked here before anything is launched. A bad one is
+// refused with its name whatever device it lies on; tensors on a device other
+// than CUDA are refused last, and so is one that requires a gradient. The GIL
+// is released during the call.
+#include <Python.h>
+
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <ATen/record_function.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/library.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
 
 #include <climits>
+#include <cstdlib>
 #include <initializer_list>
 #include <optional>
 #include <tuple>
@@ -165,7 +177,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
 }
 
 // out: null for a new tensor
-at::Tensor rope_append_paged_to(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
+at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
                                 const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
                                 at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
                                 double eps, bool interleaved, const at::Tensor* given) {
@@ -238,23 +250,7 @@ at::Tensor rope_append_paged_to(const at::Tensor& qkv, const at::Tensor& cos, co
   return out;
 }
 
-at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
-                             const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
-                             at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
-                             double eps, bool interleaved) {
-  return rope_append_paged_to(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
-                              interleaved, nullptr);
-}
-
-void rope_append_paged_out(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
-                           const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
-                           at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
-                           double eps, bool interleaved, at::Tensor& out) {
-  rope_append_paged_to(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps, interleaved,
-                       &out);
-}
-
-at::Tensor paged_attention_to(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
                               const at::Tensor& block_tables, const at::Tensor& lengths, double scale,
                               const at::Tensor* given) {
   constexpr const char* op = "paged_attention";
@@ -312,16 +308,6 @@ at::Tensor paged_attention_to(const at::Tensor& q, const at::Tensor& k_pages, co
   return out;
 }
 
-at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                           const at::Tensor& block_tables, const at::Tensor& lengths, double scale) {
-  return paged_attention_to(q, k_pages, v_pages, block_tables, lengths, scale, nullptr);
-}
-
-void paged_attention_out(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                         const at::Tensor& block_tables, const at::Tensor& lengths, double scale, at::Tensor& out) {
-  paged_attention_to(q, k_pages, v_pages, block_tables, lengths, scale, &out);
-}
-
 using LogprobsResult = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
 LogprobsResult token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t top_k,
@@ -369,27 +355,155 @@ LogprobsResult token_logprobs(const at::Tensor& logits, const at::Tensor& tokens
   return {logprob, entropy, lse, top_logprobs, top_tokens, top_logits};
 }
 
+// ------------------------------------------------------ Python side --
+// The positional arguments of a call, taken one after the other.
+class Args {
+ public:
+  Args(const char* op, PyObject* const* args, Py_ssize_t n, Py_ssize_t wanted) : op_(op), args_(args) {
+    TORCH_CHECK_TYPE(n == wanted, op, " takes ", wanted, " arguments, got ", n);
+  }
+  const at::Tensor& tensor(const char* name) {
+    PyObject* o = args_[i_++];
+    TORCH_CHECK_TYPE(THPVariable_Check(o), op_, ": ", name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+  }
+  OptTensor optional_tensor(const char* name) {
+    if (args_[i_] == Py_None) {
+      ++i_;
+      return std::nullopt;
+    }
+    return tensor(name);
+  }
+  int64_t integer(const char* name) {
+    PyObject* o = args_[i_++];
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) refuse(name, "a 64-bit integer", o);
+    return v;
+  }
+  double number(const char* name) {
+    PyObject* o = args_[i_++];
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) refuse(name, "a number", o);
+    return v;
+  }
+  bool truth() {
+    const int v = PyObject_IsTrue(args_[i_++]);
+    if (v < 0) throw python_error();
+    return v != 0;
+  }
+
+ private:
+  void refuse(const char* name, const char* what, PyObject* o) {
+    PyErr_Clear();
+    TORCH_CHECK_TYPE(false, op_, ": ", name, " must be ", what, ", got ", Py_TYPE(o)->tp_name);
+  }
+  const char* op_;
+  PyObject* const* args_;
+  Py_ssize_t i_ = 0;
+};
+
+// Runs f without the GIL, as an event that profilers see.
+template <typename F>
+auto without_gil(const char* name, F&& f) {
+  struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+  } released;
+  RECORD_FUNCTION(name, std::vector<c10::IValue>{});
+  return f();
+}
+
+template <typename... T>
+PyObject* tuple_of(const std::tuple<T...>& tensors) {
+  PyObject* r = PyTuple_New(sizeof...(T));
+  if (r == nullptr) throw python_error();
+  Py_ssize_t i = 0;
+  std::apply([&](const auto&... t) { (PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t)), ...); }, tensors);
+  return r;
+}
+
+PyObject* py_assign_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("assign_pages", args, n, 7);
+  const at::Tensor& cached = a.tensor("cached");
+  const OptTensor query_start = a.optional_tensor("query_start");
+  at::Tensor block_tables = a.tensor("block_tables");
+  const at::Tensor &free_pages = a.tensor("free_pages"), &taken = a.tensor("taken");
+  const int64_t page_size = a.integer("page_size"), num_tokens = a.integer("num_tokens");
+  return tuple_of(without_gil("nab::assign_pages", [&] {
+    return assign_pages(cached, query_start, block_tables, free_pages, taken, page_size, num_tokens);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("rope_append_paged", args, n, 13);
+  const at::Tensor &qkv = a.tensor("qkv"), &cos = a.tensor("cos"), &sin = a.tensor("sin");
+  const at::Tensor &positions = a.tensor("positions"), &slots = a.tensor("slots");
+  at::Tensor k_pages = a.tensor("k_pages"), v_pages = a.tensor("v_pages");
+  const int64_t q_heads = a.integer("q_heads");
+  const OptTensor q_norm = a.optional_tensor("q_norm"), k_norm = a.optional_tensor("k_norm");
+  const double eps = a.number("eps");
+  const bool interleaved = a.truth();
+  const OptTensor out = a.optional_tensor("out");
+  return THPVariable_Wrap(without_gil("nab::rope_append_paged", [&] {
+    return rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
+                             interleaved, out ? &*out : nullptr);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("paged_attention", args, n, 7);
+  const at::Tensor &q = a.tensor("q"), &k_pages = a.tensor("k_pages"), &v_pages = a.tensor("v_pages");
+  const at::Tensor &block_tables = a.tensor("block_tables"), &lengths = a.tensor("lengths");
+  const double scale = a.number("scale");
+  const OptTensor out = a.optional_tensor("out");
+  return THPVariable_Wrap(without_gil("nab::paged_attention", [&] {
+    return paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out ? &*out : nullptr);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("token_logprobs", args, n, 4);
+  const at::Tensor &logits = a.tensor("logits"), &tokens = a.tensor("tokens");
+  const int64_t top_k = a.integer("top_k"), vocab_start = a.integer("vocab_start");
+  return tuple_of(
+      without_gil("nab::token_logprobs", [&] { return token_logprobs(logits, tokens, top_k, vocab_start); }));
+  END_HANDLE_TH_ERRORS
+}
+
+// Whether NAB_CHECK asks for a check after every launch (os.environ's changes reach getenv).
+PyObject* py_check_requested(PyObject*, PyObject*) {
+  const char* v = std::getenv("NAB_CHECK");
+  if (v == nullptr || *v == '\0') Py_RETURN_FALSE;
+  Py_RETURN_TRUE;  // any value: the caller reads it
+}
+
+template <typename F>
+PyCFunction method(F* f) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+
+PyMethodDef kMethods[] = {
+    {"assign_pages", method(py_assign_pages), METH_FASTCALL,
+     "assign_pages(cached, query_start, block_tables, free_pages, taken, page_size, num_tokens)"},
+    {"rope_append_paged", method(py_rope_append_paged), METH_FASTCALL,
+     "rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps, interleaved, "
+     "out)"},
+    {"paged_attention", method(py_paged_attention), METH_FASTCALL,
+     "paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out)"},
+    {"token_logprobs", method(py_token_logprobs), METH_FASTCALL, "token_logprobs(logits, tokens, top_k, vocab_start)"},
+    {"check_requested", method(py_check_requested), METH_NOARGS, "whether NAB_CHECK is set"},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_C", "Serving operators; the other ops are torch.ops.nab.*", -1,
+                       kMethods,              nullptr, nullptr, nullptr, nullptr};
+
 }  // namespace
 
-TORCH_LIBRARY_FRAGMENT(nab, m) {
-  constexpr auto any = c10::DispatchKey::CompositeImplicitAutograd;
-  m.def("assign_pages(Tensor cached, Tensor? query_start, Tensor(a!) block_tables, Tensor free_pages, Tensor taken, "
-        "int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.impl("assign_pages", torch::dispatch(any, TORCH_FN(assign_pages)));
-  m.def("rope_append_paged(Tensor qkv, Tensor cos, Tensor sin, Tensor positions, Tensor slots, Tensor(a!) k_pages, "
-        "Tensor(b!) v_pages, int q_heads, Tensor? q_norm, Tensor? k_norm, float eps, bool interleaved) -> Tensor");
-  m.impl("rope_append_paged", torch::dispatch(any, TORCH_FN(rope_append_paged)));
-  m.def("rope_append_paged.out(Tensor qkv, Tensor cos, Tensor sin, Tensor positions, Tensor slots, "
-        "Tensor(a!) k_pages, Tensor(b!) v_pages, int q_heads, Tensor? q_norm, Tensor? k_norm, float eps, "
-        "bool interleaved, Tensor(c!) out) -> ()");
-  m.impl("rope_append_paged.out", torch::dispatch(any, TORCH_FN(rope_append_paged_out)));
-  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, "
-        "float scale) -> Tensor");
-  m.impl("paged_attention", torch::dispatch(any, TORCH_FN(paged_attention)));
-  m.def("paged_attention.out(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, "
-        "float scale, Tensor(a!) out) -> ()");
-  m.impl("paged_attention.out", torch::dispatch(any, TORCH_FN(paged_attention_out)));
-  m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k, int vocab_start) -> "
-        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.impl("token_logprobs", torch::dispatch(any, TORCH_FN(token_logprobs)));
-}
+PyMODINIT_FUNC PyInit__C() { return PyModule_Create(&kModule); }

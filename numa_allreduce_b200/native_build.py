@@ -2,8 +2,9 @@
 
 Produces two shared objects next to this file:
 
-* ``_C.so``     the core plus the torch op bindings (``torch.ops.nab.*``),
-                linked against torch and the CUDA runtime torch already loads;
+* ``_C.so``     the core plus the torch op bindings (``torch.ops.nab.*``, and
+                the Python module ``_C`` of the serving operators), linked
+                against torch and the CUDA runtime torch already loads;
 * ``libnab.so`` the core plus the plain C ABI, with the CUDA runtime linked
                 statically, for callers that do not use Python or torch.
 
@@ -21,6 +22,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -68,7 +70,7 @@ def _torch_flags() -> tuple[list[str], list[str], str]:
     import torch
     from torch.utils import cpp_extension
 
-    incs = [f"-I{p}" for p in cpp_extension.include_paths()]
+    incs = [f"-I{p}" for p in cpp_extension.include_paths()] + [f"-I{sysconfig.get_paths()['include']}"]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     lib_dir = str(Path(torch.__file__).resolve().parent / "lib")
     return incs, [f"-D_GLIBCXX_USE_CXX11_ABI={abi}"], lib_dir
@@ -170,7 +172,7 @@ def build(verbose: bool = False, jobs: int | None = None, debug: bool = False) -
     cuda_lib = str(cuda / "lib64")
     torch_out = DEBUG_TORCH_LIB if debug else TORCH_LIB
     _link(torch_out, core + tobj,
-          [f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda",
+          [f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda", "-ltorch_python",
            f"-L{cuda_lib}", "-lcudart", f"-Wl,-rpath,{torch_lib}"], verbose)
     if debug:
         return {"torch": str(torch_out)}

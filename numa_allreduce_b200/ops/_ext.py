@@ -11,6 +11,8 @@ device-side bounds checks compiled in (slower; for tests and debugging).
 
 from __future__ import annotations
 
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -19,6 +21,7 @@ import torch
 
 _LOCK = threading.Lock()
 _LOADED: str | None = None
+_NATIVE = None
 
 
 def _debug() -> bool:
@@ -53,6 +56,20 @@ def load():
         torch.ops.load_library(str(path))
         _LOADED = str(path)
     return torch.ops.nab
+
+
+def native():
+    """The library as a Python module: the operators that are bound directly,
+    without torch's dispatcher (a call through it takes 2.4 us longer)."""
+    global _NATIVE
+    if _NATIVE is None:
+        load()
+        loader = importlib.machinery.ExtensionFileLoader(__package__.rpartition(".")[0] + "._C", _LOADED)
+        spec = importlib.util.spec_from_file_location(loader.name, _LOADED, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _NATIVE = module
+    return _NATIVE
 
 
 def loaded_path() -> str | None:

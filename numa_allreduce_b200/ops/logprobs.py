@@ -36,9 +36,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, v
     :func:`join_token_logprobs` makes the whole vocabulary's from all shards.
     For inference: logits that require a gradient are refused.
     """
-    ops = _ext.load()
-    r = TokenLogprobs._make(ops.token_logprobs.default(logits, tokens, top_k, vocab_start))
-    after_launch()
+    native = _ext.native()
+    r = TokenLogprobs._make(native.token_logprobs(logits, tokens, top_k, vocab_start))
+    if native.check_requested():
+        after_launch()
     return r
 
 

@@ -58,14 +58,15 @@ def assign_pages(cached: torch.Tensor, block_tables: torch.Tensor, free_pages: t
     ``lengths[b] < cached[b] + new tokens`` tells it. ``cached`` and ``taken``
     are not changed.
     """
-    ops = _ext.load()
+    native = _ext.native()
     if num_tokens is None:
         if query_start is not None:
             raise ValueError("assign_pages needs num_tokens with query_start")
         num_tokens = cached.shape[0]
-    r = PageSlots._make(ops.assign_pages.default(cached, query_start, block_tables, free_pages, taken, page_size,
-                                                 num_tokens))
-    after_launch()
+    r = PageSlots._make(native.assign_pages(cached, query_start, block_tables, free_pages, taken, page_size,
+                                            num_tokens))
+    if native.check_requested():
+        after_launch()
     return r
 
 
@@ -91,15 +92,12 @@ def rope_append_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
     (:func:`~numa_allreduce_b200.check_kernels`). Returns q as
     ``[tokens, q_heads, head_dim]``.
     """
-    ops = _ext.load()
-    if out is None:
-        out = ops.rope_append_paged.default(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm,
-                                            eps, interleaved)
-    else:
-        ops.rope_append_paged.out(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
-                                  interleaved, out)
-    after_launch()
-    return out
+    native = _ext.native()
+    q = native.rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
+                                 interleaved, out)
+    if native.check_requested():
+        after_launch()
+    return q
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
@@ -119,14 +117,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     The work of all requests is split evenly over the GPU, so long and short
     requests may be mixed; parts of a request are joined in a second launch.
     """
-    ops = _ext.load()
+    native = _ext.native()
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if out is None:
-        out = ops.paged_attention.default(q, k_pages, v_pages, block_tables, lengths, scale)
-    else:
-        ops.paged_attention.out(q, k_pages, v_pages, block_tables, lengths, scale, out)
-    after_launch()
+    out = native.paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out)
+    if native.check_requested():
+        after_launch()
     return out
 
 

@@ -12,6 +12,7 @@ Tolerances. u = finfo(type).eps / 2 is the error of one rounding to the
   a factor 1 +- 2 d; the sums over n positions add (n / 64 + 64) 2^-22 A.
 """
 
+import concurrent.futures
 import math
 
 import pytest
@@ -629,3 +630,21 @@ def test_another_stream():
         out = nab.paged_attention(q, k, v, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
         check_attention(out, q, k, v, tables, lengths, 128 ** -0.5)
     torch.cuda.synchronize()
+
+
+def test_calls_from_several_threads():
+    def work(seed):
+        lengths = [300 + 7 * seed, 0, 33]
+        k, v, tables = make_cache(lengths, 2, 64, 16, BF, seed=seed)
+        q = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(seed)).to("cuda", BF)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [nab.paged_attention(q, k, v, tables, n) for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+        return outs, q, k, v, tables, lengths
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for outs, q, k, v, tables, lengths in pool.map(work, range(4)):
+            check_attention(outs[0], q, k, v, tables, lengths, 64 ** -0.5)
+            assert all(torch.equal(o, outs[0]) for o in outs[1:])

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import numa_allreduce_b200 as nab
+from numa_allreduce_b200.ops import _ext
 
 
 def _i32(*v):
@@ -276,3 +277,22 @@ def test_decoder_refuses(kw, match):
 
     with pytest.raises(ValueError, match=match):
         LlamaTPDecoder(LlamaConfig.tiny(), None, batch=1, context=4, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("call, match", [
+    (lambda n, t: n.token_logprobs(None, t, 1, 0), "token_logprobs: logits must be a tensor, got NoneType"),
+    (lambda n, t: n.token_logprobs(t, [1], 1, 0), "token_logprobs: tokens must be a tensor, got list"),
+    (lambda n, t: n.token_logprobs(t, t, 1.5, 0), "token_logprobs: top_k must be a 64-bit integer, got float"),
+    (lambda n, t: n.token_logprobs(t, t, 1 << 70, 0), "token_logprobs: top_k must be a 64-bit integer, got int"),
+    (lambda n, t: n.token_logprobs(t, t, 1), "token_logprobs takes 4 arguments, got 3"),
+    (lambda n, t: n.token_logprobs(), "token_logprobs takes 4 arguments, got 0"),
+    (lambda n, t: n.paged_attention(t, t, t, t, t, "1", None), "paged_attention: scale must be a number, got str"),
+    (lambda n, t: n.paged_attention(t, t, t, t, t, 1, 2), "paged_attention: out must be a tensor, got int"),
+    (lambda n, t: n.assign_pages(t, 3, t, t, t, 16, 1), "assign_pages: query_start must be a tensor, got int"),
+    (lambda n, t: n.assign_pages(t, None, t, t, t, 16, None), "assign_pages: num_tokens must be a 64-bit integer"),
+    (lambda n, t: n.rope_append_paged(t, t, t, t, t, t, "v", 1, None, None, 0.0, False, None),
+     "rope_append_paged: v_pages must be a tensor, got str"),
+])
+def test_arguments_of_the_wrong_kind(call, match):
+    with pytest.raises(TypeError, match=match):
+        call(_ext.native(), torch.zeros(1))
