@@ -222,6 +222,8 @@ __global__ void __launch_bounds__(kPThreads, 2)
     misc[1] = a.B;
     sm100::prefetch_tensormap(&tk);
     sm100::prefetch_tensormap(&tv);
+    sm100::prefetch_tensormap(&tk16);
+    sm100::prefetch_tensormap(&tv16);
     sm100::prefetch_tensormap(&tq);
   }
   pdl_wait();
@@ -229,10 +231,13 @@ __global__ void __launch_bounds__(kPThreads, 2)
 
   Walk w;
   int per = 1, lo = 0;  // units per CTA, first unit of this one's range
+  int early = 0;        // cluster form, fetching warp: lane i's is page i of the request
   if constexpr (kCluster) {
     const int segment = static_cast<int>(blockIdx.x) / a.cluster, rank = static_cast<int>(blockIdx.x) % a.cluster;
     w.b = segment / HH;
     w.h = segment % HH;
+    // loaded beside the length, which says only then which of them count
+    if (warp == kWarps && lane < a.M) early = __ldg(a.tables + w.b * a.table_stride + lane);
     const int raw = a.lengths[w.b];
     if (tid == 0 && rank == 0 && w.h == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
       record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(w.b));
@@ -349,9 +354,13 @@ __global__ void __launch_bounds__(kPThreads, 2)
     };
     bool more = w.x < w.x1, given_up = false;
     if (more) {
-      window = static_cast<int>(static_cast<int64_t>(w.t) * kTile / a.P);
-      ids = load_ids(w.b, window);
-      ahead = load_ids(w.b + 1, 0);
+      if constexpr (kCluster) {
+        ids = early;
+      } else {
+        window = static_cast<int>(static_cast<int64_t>(w.t) * kTile / a.P);
+        ids = load_ids(w.b, window);
+        ahead = load_ids(w.b + 1, 0);
+      }
     }
     while (more) {
       const int n = tiles_here();
