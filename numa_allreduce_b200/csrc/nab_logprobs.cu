@@ -18,9 +18,9 @@
 // counting. If a contrived row overflows the collection, k rounds of a block
 // maximum over the same pieces replace it.
 //
-// A row is shared by a thread-block cluster of 1 to 8 CTAs, joined by its
-// first CTA over distributed shared memory: one launch, no workspace, and a
-// fixed order of additions.
+// A row is shared by a thread-block cluster of 1 to 8 CTAs, which write their
+// results into the first one's shared memory for it to join: one launch, no
+// workspace, and a fixed order of additions.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -44,7 +44,7 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 1024;  // collected elements of a CTA
 constexpr int kSub = 8;      // parts of a thread's share
-constexpr int kPad = 24 * 1024;  // beside the static 35 KB: three CTAs per SM
+constexpr int kPad = 24 * 1024;  // beside the static 37 KB: three CTAs per SM
 constexpr int kCoarse = 64;  // parts that give the cut: the threads of one remainder mod 64
 constexpr float kL2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -203,8 +203,9 @@ NAB_DINLINE void raise(Stats& a, float m) {
 
 struct LpShared {
   float warp_m[kLpWarps], warp_s[kLpWarps], warp_u[kLpWarps];
-  Stats stats;                          // this CTA's, read by the cluster's first CTA
-  uint64_t top[kMaxTopK];               // this CTA's largest keys, in order; 0 past its elements
+  // of each CTA of the cluster, written by that one into the first one's memory:
+  Stats stats[kMaxCluster];
+  uint64_t top[kMaxCluster * kMaxTopK]; // k largest keys, in order; 0 past its elements
   uint64_t cand[kCand];
   float2 part[kSub * kLpThreads];       // of each part: its maximum, and as bits the first piece that holds it
   uint64_t best[kLpThreads];            // (value, piece) of each thread's largest, 0 without pieces
@@ -251,9 +252,13 @@ struct Row {
   NAB_DINLINE uint4 whole(int p) const { return ld_plain(x + first(p)); }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster) {
+// kCluster: rows are shared by clusters. Compiled apart: 1023 rows of one CTA each 52.5 -> 51.8 us, and 32 rows of
+// 4 CTAs 5.6 -> 5.5 (5.9 when the first CTA read the others' results over the cluster).
+template <typename T, bool kCluster>
+__global__ void __launch_bounds__(kLpThreads, 4)
+    k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster_size) {
   __shared__ LpShared sh;
+  const int cluster = kCluster ? cluster_size : 1;
   constexpr int N = Row<T>::kN;
   constexpr int kBatch = 4;
   pdl_wait();
@@ -270,13 +275,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   const int p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);  // this CTA's pieces
   const int i0 = max(p0, r.mis > 0), i1 = min(p1, (r.mis + a.V) / N);  // those within the row
   const int k = a.top_k;
-  float picked = 0.f;  // the given token's logit, if it is in this part of the vocabulary
-  bool here = false;
-  if (tid == 0 && part == 0) {
-    const int64_t token = a.tokens[row];  // any value
-    here = token >= a.vocab_start && token - a.vocab_start < a.V;
-    if (here) picked = static_cast<float>(r.x[token - a.vocab_start]);
-  }
+  if (part == 0)
+    for (int i = tid; i < cluster * k; i += kLpThreads) sh.top[i] = 0;
+  if constexpr (kCluster) sm100::cluster_arrive();
 
   // ------------------------------------------------------- one pass --
   // Piece p is thread (p - p0) % kLpThreads's. Batches of kBatch pieces, the
@@ -302,6 +303,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   for (int b = 0; b < kBatch; ++b) {
     const int q = p + b * kLpThreads;
     cur[b] = q >= i0 && q < i1 ? at[b * kLpThreads] : fill;
+  }
+  // (behind the first loads: a token's logit waits for its index)
+  float picked = 0.f;  // the given token's logit, if it is in this part of the vocabulary
+  bool here = false;
+  if (tid == 0 && part == 0) {
+    const int64_t token = a.tokens[row];  // any value
+    here = token >= a.vocab_start && token - a.vocab_start < a.V;
+    if (here) picked = static_cast<float>(r.x[token - a.vocab_start]);
   }
   for (int j = 0; j < batches; ++j) {
     uint4 next[kBatch];
@@ -385,7 +394,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) sh.warp_m[warp] = top;
   sh.best[tid] = p0 + tid < p1 ? piece_key(st.m, big_at) : 0;
-  if (tid < kMaxTopK) sh.top[tid] = 0;
   if (tid < kCoarse) sh.coarse_rank[tid] = 0;
   if (tid == 0) {
     sh.n_who = sh.n_cand = 0;
@@ -406,7 +414,25 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   raise<T>(st, top);
   const float2 sums = block_sum(make_float2(st.s, st.u), sh.warp_s, sh.warp_u);
-  if (tid == 0) sh.stats = {top, sums.x, sums.y};
+  // where the first CTA takes this one's results from; it has started
+  uint32_t stats_at = 0, top_at = 0;
+  if constexpr (kCluster) {
+    sm100::cluster_wait();
+    stats_at = sm100::dsmem_addr(sm100::smem_u32(&sh.stats[part]), 0);
+    top_at = sm100::dsmem_addr(sm100::smem_u32(&sh.top[part * k]), 0);
+  }
+  auto put = [&](int rank, uint64_t key) {
+    if constexpr (kCluster) sm100::st_dsmem_u64(top_at + rank * 8, key); else sh.top[rank] = key;
+  };
+  if (tid == 0) {
+    if constexpr (kCluster) {
+      sm100::st_dsmem_f32(stats_at, top);
+      sm100::st_dsmem_f32(stats_at + 4, sums.x);
+      sm100::st_dsmem_f32(stats_at + 8, sums.y);
+    } else {
+      sh.stats[0] = {top, sums.x, sums.y};
+    }
+  }
 
   // ------------------------------------------------------ top k of the CTA --
   if (k > 0) {
@@ -465,7 +491,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
         const uint64_t mine = sh.cand[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine;
-        if (rank < k) sh.top[rank] = mine;
+        if (rank < k) put(rank, mine);
       }
     } else {
       uint64_t last = ~uint64_t{0};
@@ -482,7 +508,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
         if (lane == 0) sh.best[warp] = next;
         __syncthreads();
         for (int w = 0; w < kLpWarps; ++w) next = sh.best[w] > next ? sh.best[w] : next;
-        if (tid == 0) sh.top[i] = next;
+        if (tid == 0) put(i, next);
         last = next;
         __syncthreads();
       }
@@ -490,37 +516,24 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
   }
 
   // ---------------------------------------------------- join of the cluster --
-  if (cluster > 1) sm100::cluster_sync(); else __syncthreads();
+  if constexpr (kCluster) sm100::cluster_sync(); else __syncthreads();
   if (part == 0) {
-    Stats all = sh.stats;
-    uint64_t mine = 0;
-    if (cluster > 1) {
+    Stats all = sh.stats[0];
+    // keys of every CTA, one per thread; all are different
+    static_assert(kMaxCluster * kMaxTopK <= kLpThreads, "one key per thread");
+    const uint64_t mine = tid < cluster * k ? sh.top[tid] : 0;
+    if constexpr (kCluster) {
       // every thread adds the CTAs up for itself, in their order
-      Stats part_[kMaxCluster];
-#pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c) {
-        const uint32_t at = sm100::dsmem_addr(sm100::smem_u32(&sh.stats), c < cluster ? c : 0);
-        part_[c] = {sm100::ld_dsmem_f32(at), sm100::ld_dsmem_f32(at + 4), sm100::ld_dsmem_f32(at + 8)};
-        all.m = fmaxf(all.m, part_[c].m);
-      }
-      // keys of every CTA, one per thread (8 x 32 at most); all are different
-      static_assert(kMaxCluster * kMaxTopK <= kLpThreads && kMaxCluster * kMaxTopK <= kCand, "one key per thread");
-      if (tid < cluster * k) {
-        const uint32_t at = sm100::dsmem_addr(sm100::smem_u32(&sh.top[tid % k]), tid / k);
-        const uint32_t lo = __float_as_uint(sm100::ld_dsmem_f32(at)), hi = __float_as_uint(sm100::ld_dsmem_f32(at + 4));
-        mine = (static_cast<uint64_t>(hi) << 32) | lo;
-      }
-      if (tid < kMaxCluster * kMaxTopK) sh.cand[tid] = mine;
+      for (int c = 1; c < cluster; ++c) all.m = fmaxf(all.m, sh.stats[c].m);
       all.s = all.u = 0.f;
 #pragma unroll
       for (int c = 0; c < kMaxCluster; ++c) {
-        raise<T>(part_[c], all.m);
-        all.s += c < cluster ? part_[c].s : 0.f;
-        all.u += c < cluster ? part_[c].u : 0.f;
+        if (c >= cluster) break;
+        Stats one = sh.stats[c];
+        raise<T>(one, all.m);
+        all.s += one.s;
+        all.u += one.u;
       }
-      __syncthreads();
-    } else if (tid < k) {
-      mine = sh.top[tid];
     }
     const bool far = all.m > Piece<T>::kHigh || all.m < Piece<T>::kLow;
     if (all.m == -INFINITY && all.s == all.s) all.s = all.u = 0.f;  // nothing but -inf
@@ -549,9 +562,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
     }
     if (mine != 0) {
       int rank = tid;
-      if (cluster > 1) {
+      if constexpr (kCluster) {
         rank = 0;
-        for (int j = 0; j < cluster * k; ++j) rank += sh.cand[j] > mine;
+        for (int j = 0; j < cluster * k; ++j) rank += sh.top[j] > mine;
       }
       if (rank < k) {
         const float x = unordered(static_cast<uint32_t>(mine >> 32));
@@ -561,7 +574,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_token_logprobs(const __grid_c
       }
     }
   }
-  if (cluster > 1) sm100::cluster_sync();  // the first CTA has read the others
 }
 
 template <typename T>
@@ -580,13 +592,14 @@ void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
   cfg.blockDim = dim3(kLpThreads);
   cfg.stream = s;
   // Four CTAs fit on an SM; of a grid that fills two to three per SM some SMs would get four and others two. Shared
-  // memory that nobody uses makes it three: 300 x 128256 bf16 30.7 -> 25.2 us.
+  // memory that nobody uses makes it three: 300 x 128256 bf16 30.7 -> 25.2 us. (Clusters have up to two per SM.)
   if (grid > 2 * sms && grid <= 3 * sms) cfg.dynamicSmemBytes = kPad;
+  const auto kernel = cluster > 1 ? k_token_logprobs<T, true> : k_token_logprobs<T, false>;
   static std::atomic<bool> ready[64];  // by device; setting it twice does no harm
   int dev = 0;
   NAB_CUDA_CHECK(cudaGetDevice(&dev));
   if (cfg.dynamicSmemBytes > 0 && !ready[dev & 63].load(std::memory_order_acquire)) {
-    NAB_CUDA_CHECK(cudaFuncSetAttribute(k_token_logprobs<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPad));
+    NAB_CUDA_CHECK(cudaFuncSetAttribute(k_token_logprobs<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPad));
     ready[dev & 63].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute attrs[2];
@@ -598,7 +611,7 @@ void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
   attrs[1].val.clusterDim.z = 1;
   cfg.attrs = attrs;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_token_logprobs<T>, a, cluster);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, cluster);
   if (e != cudaSuccess) throw std::runtime_error(std::string("token_logprobs launch failed: ") + cudaGetErrorString(e));
 }
 

@@ -143,6 +143,9 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(int m, int n) {
 NAB_DINLINE void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The same in two halves: what a thread writes before its arrival is seen by every thread that has waited.
+NAB_DINLINE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+NAB_DINLINE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 NAB_DINLINE uint32_t cluster_ctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -158,6 +161,12 @@ NAB_DINLINE float ld_dsmem_f32(uint32_t cluster_addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
   return v;
+}
+NAB_DINLINE void st_dsmem_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+NAB_DINLINE void st_dsmem_u64(uint32_t cluster_addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_addr), "l"(v) : "memory");
 }
 NAB_DINLINE float4 ld_dsmem_f4(uint32_t cluster_addr) {
   float4 v;
