@@ -8,15 +8,15 @@
 //
 // One pass over the row with a running (m, S, sum) per thread, so each logit
 // is read from HBM once. The top k cost no second pass over the row: each
-// thread notes, for each eighth of its share, the maximum and the first
-// 16-byte piece that held it. Take any partition of the row and order its
-// parts by (maximum, piece): an element of the top k can only lie in a part
-// whose key reaches the k-th of these keys, since each part before it holds
-// an element that precedes it. The k-th of 64 coarse parts is a cut; the
-// eighths that reach it (about 1.2 k of them) are read again, from L2, and
-// the elements that reach it are collected in shared memory and ranked by
-// counting. If a contrived row overflows the collection, k rounds of a block
-// maximum over the same pieces replace it.
+// thread notes, for each part of its share (an eighth, or a quarter), the
+// maximum and the first 16-byte piece that held it. Take any partition of the
+// row and order its parts by (maximum, piece): an element of the top k can
+// only lie in a part whose key reaches the k-th of these keys, since each part
+// before it holds an element that precedes it. The k-th of 64 coarse parts is
+// a cut; the parts that reach it (about 1.2 k of them) are read again, from
+// L2, and the elements that reach it are collected in shared memory and ranked
+// by counting. If a contrived row overflows the collection, k rounds of a
+// block maximum over the same pieces replace it.
 //
 // A row is shared by a thread-block cluster of 1 to 8 CTAs, which write their
 // results into the first one's shared memory for it to join: one launch, no
@@ -39,12 +39,10 @@ namespace nab {
 
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 1024;  // collected elements of a CTA
-constexpr int kSub = 8;      // parts of a thread's share
-constexpr int kPad = 24 * 1024;  // beside the static 37 KB: three CTAs per SM
+constexpr int kParts = 2048;  // parts of a CTA's share
+constexpr int kPad = 24 * 1024;  // beside the static 37 KB of 256 threads: three CTAs per SM
 constexpr int kCoarse = 64;  // parts that give the cut: the threads of one remainder mod 64
 constexpr float kL2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -201,22 +199,24 @@ NAB_DINLINE void raise(Stats& a, float m) {
   a.m = m;
 }
 
+template <int kThreads>
 struct LpShared {
-  float warp_m[kLpWarps], warp_s[kLpWarps], warp_u[kLpWarps];
+  float warp_m[kThreads / 32], warp_s[kThreads / 32], warp_u[kThreads / 32];
   // of each CTA of the cluster, written by that one into the first one's memory:
   Stats stats[kMaxCluster];
   uint64_t top[kMaxCluster * kMaxTopK]; // k largest keys, in order; 0 past its elements
   uint64_t cand[kCand];
-  float2 part[kSub * kLpThreads];       // of each part: its maximum, and as bits the first piece that holds it
-  uint64_t best[kLpThreads];            // (value, piece) of each thread's largest, 0 without pieces
+  float2 part[kParts];       // of each part: its maximum, and as bits the first piece that holds it
+  uint64_t best[kThreads];            // (value, piece) of each thread's largest, 0 without pieces
   uint64_t coarse[kCoarse];
   int coarse_rank[kCoarse];
   uint64_t cut;
-  int who[kSub * kLpThreads];           // parts that are read again
+  int who[kParts];           // parts that are read again
   int n_who, n_cand;
 };
 
 // Sum over the block, for every thread, in a fixed order; a and b are used again after the next barrier.
+template <int kWarps>
 NAB_DINLINE float2 block_sum(float2 v, float* a, float* b) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
@@ -229,9 +229,9 @@ NAB_DINLINE float2 block_sum(float2 v, float* a, float* b) {
     b[warp] = v.y;
   }
   __syncthreads();
-  v = lane < kLpWarps ? make_float2(a[lane], b[lane]) : make_float2(0.f, 0.f);
+  v = lane < kWarps ? make_float2(a[lane], b[lane]) : make_float2(0.f, 0.f);
 #pragma unroll
-  for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+  for (int o = kWarps / 2; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
@@ -252,12 +252,13 @@ struct Row {
   NAB_DINLINE uint4 whole(int p) const { return ld_plain(x + first(p)); }
 };
 
-// kCluster: rows are shared by clusters. Compiled apart: 1023 rows of one CTA each 52.5 -> 51.8 us, and 32 rows of
-// 4 CTAs 5.6 -> 5.5 (5.9 when the first CTA read the others' results over the cluster).
-template <typename T, bool kCluster>
-__global__ void __launch_bounds__(kLpThreads, 4)
+// kCluster: rows are shared by clusters. Compiled apart: 1023 rows of one CTA each 52.5 -> 51.8 us.
+template <typename T, bool kCluster, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     k_token_logprobs(const __grid_constant__ LogprobsArgs a, int cluster_size) {
-  __shared__ LpShared sh;
+  __shared__ LpShared<kThreads> sh;
+  constexpr int kWarps = kThreads / 32;
+  constexpr int kSub = kParts / kThreads;  // parts of a thread's share
   const int cluster = kCluster ? cluster_size : 1;
   constexpr int N = Row<T>::kN;
   constexpr int kBatch = 4;
@@ -276,14 +277,14 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   const int i0 = max(p0, r.mis > 0), i1 = min(p1, (r.mis + a.V) / N);  // those within the row
   const int k = a.top_k;
   if (part == 0)
-    for (int i = tid; i < cluster * k; i += kLpThreads) sh.top[i] = 0;
+    for (int i = tid; i < cluster * k; i += kThreads) sh.top[i] = 0;
   if constexpr (kCluster) sm100::cluster_arrive();
 
   // ------------------------------------------------------- one pass --
-  // Piece p is thread (p - p0) % kLpThreads's. Batches of kBatch pieces, the
+  // Piece p is thread (p - p0) % kThreads's. Batches of kBatch pieces, the
   // next one's loads in flight during one's arithmetic; pieces past the end
   // read as -inf, i.e. as elements of probability 0.
-  const int batches = ((p1 - p0 + kLpThreads - 1) / kLpThreads + kBatch - 1) / kBatch;
+  const int batches = ((p1 - p0 + kThreads - 1) / kThreads + kBatch - 1) / kBatch;
   const int sub_batches = max(1, (batches + kSub - 1) / kSub);
   // (value, piece within the CTA), larger = earlier, in as few bits as it takes
   const int piece_bits = 32 - __clz(p1 - p0);
@@ -301,8 +302,8 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   uint4 cur[kBatch];
 #pragma unroll
   for (int b = 0; b < kBatch; ++b) {
-    const int q = p + b * kLpThreads;
-    cur[b] = q >= i0 && q < i1 ? at[b * kLpThreads] : fill;
+    const int q = p + b * kThreads;
+    cur[b] = q >= i0 && q < i1 ? at[b * kThreads] : fill;
   }
   // (behind the first loads: a token's logit waits for its index)
   float picked = 0.f;  // the given token's logit, if it is in this part of the vocabulary
@@ -314,18 +315,18 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   }
   for (int j = 0; j < batches; ++j) {
     uint4 next[kBatch];
-    at += kBatch * kLpThreads;
+    at += kBatch * kThreads;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       next[b] = fill;
-      if (p + (kBatch + b) * kLpThreads < i1) next[b] = at[b * kLpThreads];
+      if (p + (kBatch + b) * kThreads < i1) next[b] = at[b * kThreads];
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const float mx = Piece<T>::largest(cur[b]);
       if (mx > kv) {
         kv = mx;
-        kp = p + b * kLpThreads;
+        kp = p + b * kThreads;
       }
     }
     {
@@ -352,9 +353,9 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) cur[b] = next[b];
-    p += kBatch * kLpThreads;
+    p += kBatch * kThreads;
     if (--left == 0 || j + 1 == batches) {  // the end of a part
-      sh.part[sub * kLpThreads + tid] = make_float2(kv, __int_as_float(kp));
+      sh.part[sub * kThreads + tid] = make_float2(kv, __int_as_float(kp));
       if (kv > big) {
         big = kv;
         big_at = kp;
@@ -370,8 +371,8 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   Stats st = {big, s_.x + s_.y, u_.x + u_.y};
   // the row's first and last piece, where they reach past it
   auto edge = [&](int q) {
-    if (q < p0 || q >= p1 || r.inner(q) || (q - p0) % kLpThreads != tid) return;
-    float2& part_max = sh.part[(q - p0) / kLpThreads / kBatch / sub_batches * kLpThreads + tid];
+    if (q < p0 || q >= p1 || r.inner(q) || (q - p0) % kThreads != tid) return;
+    float2& part_max = sh.part[(q - p0) / kThreads / kBatch / sub_batches * kThreads + tid];
     for (int e = 0; e < N; ++e) {
       const int i = r.first(q) + e;
       if (i < 0 || i >= a.V) continue;
@@ -403,17 +404,17 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   if (tid < kCoarse) {
     uint64_t c = 0;
 #pragma unroll
-    for (int i = 0; i < kLpThreads / kCoarse; ++i) {
+    for (int i = 0; i < kThreads / kCoarse; ++i) {
       const uint64_t b = sh.best[tid + i * kCoarse];
       c = b > c ? b : c;
     }
     sh.coarse[tid] = c;
   }
-  top = sh.warp_m[lane % kLpWarps];
+  top = sh.warp_m[lane % kWarps];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   raise<T>(st, top);
-  const float2 sums = block_sum(make_float2(st.s, st.u), sh.warp_s, sh.warp_u);
+  const float2 sums = block_sum<kWarps>(make_float2(st.s, st.u), sh.warp_s, sh.warp_u);
   // where the first CTA takes this one's results from; it has started
   uint32_t stats_at = 0, top_at = 0;
   if constexpr (kCluster) {
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   // ------------------------------------------------------ top k of the CTA --
   if (k > 0) {
     {
-      constexpr int kEach = kCoarse * kCoarse / kLpThreads;  // comparisons of a thread
+      constexpr int kEach = kCoarse * kCoarse / kThreads;  // comparisons of a thread
       const int i = tid % kCoarse, from = tid / kCoarse * kEach;
       const uint64_t mine = sh.coarse[i];
       int before = 0;
@@ -451,18 +452,18 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     __syncthreads();
     const uint64_t cut = sh.cut;
     for (int i = 0; i < subs; ++i) {
-      const float2 part_max = sh.part[i * kLpThreads + tid];
+      const float2 part_max = sh.part[i * kThreads + tid];
       const int q = __float_as_int(part_max.y);
-      if (q < p1 && piece_key(part_max.x, q) >= cut) sh.who[atomicAdd(&sh.n_who, 1)] = i * kLpThreads + tid;
+      if (q < p1 && piece_key(part_max.x, q) >= cut) sh.who[atomicAdd(&sh.n_who, 1)] = i * kThreads + tid;
     }
     __syncthreads();
     const int n_who = sh.n_who;
     const int depth = kBatch * sub_batches;  // pieces of a part, at most
     const uint32_t cut_value = static_cast<uint32_t>(cut >> piece_bits);
     auto for_elements = [&](auto f) {
-      for (int i = tid; i < n_who * depth; i += kLpThreads) {
+      for (int i = tid; i < n_who * depth; i += kThreads) {
         const int part_at = sh.who[i / depth];
-        const int q = p0 + part_at % kLpThreads + (part_at / kLpThreads * depth + i % depth) * kLpThreads;
+        const int q = p0 + part_at % kThreads + (part_at / kThreads * depth + i % depth) * kThreads;
         if (q >= p1) continue;
         if (r.inner(q)) {
           const uint4 w = r.whole(q);
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     __syncthreads();
     const int n = sh.n_cand;
     if (n <= kCand) {
-      for (int i = tid; i < n; i += kLpThreads) {
+      for (int i = tid; i < n; i += kThreads) {
         const uint64_t mine = sh.cand[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine;
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         }
         if (lane == 0) sh.best[warp] = next;
         __syncthreads();
-        for (int w = 0; w < kLpWarps; ++w) next = sh.best[w] > next ? sh.best[w] : next;
+        for (int w = 0; w < kWarps; ++w) next = sh.best[w] > next ? sh.best[w] : next;
         if (tid == 0) put(i, next);
         last = next;
         __syncthreads();
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
   if (part == 0) {
     Stats all = sh.stats[0];
     // keys of every CTA, one per thread; all are different
-    static_assert(kMaxCluster * kMaxTopK <= kLpThreads, "one key per thread");
+    static_assert(kMaxCluster * kMaxTopK <= kThreads, "one key per thread");
     const uint64_t mine = tid < cluster * k ? sh.top[tid] : 0;
     if constexpr (kCluster) {
       // every thread adds the CTAs up for itself, in their order
@@ -539,13 +540,13 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     if (all.m == -INFINITY && all.s == all.s) all.s = all.u = 0.f;  // nothing but -inf
     if (far && fabsf(all.m) != INFINITY) {  // this CTA sums the row again as it stands
       float2 sum = make_float2(0.f, 0.f);
-      for (int i = tid; i < a.V; i += kLpThreads) {
+      for (int i = tid; i < a.V; i += kThreads) {
         const float d = max_nan((static_cast<float>(r.x[i]) - all.m) * kL2e, -1000.f), w = lp_ex2(d);
         sum.x += w;
         sum.y += d * w;
       }
       __syncthreads();
-      sum = block_sum(sum, sh.warp_s, sh.warp_u);
+      sum = block_sum<kWarps>(sum, sh.warp_s, sh.warp_u);
       all.s = sum.x;
       all.u = sum.y;
     }
@@ -578,28 +579,37 @@ __global__ void __launch_bounds__(kLpThreads, 4)
 
 template <typename T>
 void launch_lp(cudaStream_t s, const LogprobsArgs& a, int sms) {
-  // CTAs per row. A cluster pays for its two barriers and its slower launch, so only rows of many bytes and few
-  // of them are shared: at least 30 KB of logits per CTA, at most two CTAs per SM. Measured with 1 / 2 / 4 / 8
-  // CTAs per row (us, k = 20): 1 x 128256 bf16 11.4 / 9.4 / 7.7 / 7.5; 64 rows 15.9 / 12.5 / 11.2 / 13.5; 148 rows
-  // 16.6 / 14.8 / 21.5 / 28.5; 200 rows 18.7 / 21.1 / 24.9 / 34.3; 1 x 16032 5.1 / 5.6 / 5.9 / 6.6.
-  int cluster = 1;
+  // While every CTA can have an SM to itself, it gets 512 threads, i.e. twice the loads in flight, and few long rows are
+  // shared by clusters: at least 12000 elements per CTA while half of the SMs stay free, else 24000. Past that, 256
+  // threads, four CTAs on an SM, and no clusters, which pay for two barriers and a slower launch. Measured (us, bf16,
+  // k = 20): 256 threads with 1 / 2 / 4 / 8 CTAs per row; 512 threads: 1 x 128256 11.7 9.2 7.3 7.0; 10.2 8.6 7.4 7.2.
+  // 16 rows 15.6 11.7 9.1 8.8; 11.0 9.4 8.1 9.6. 32 rows 15.7 12.0 9.6 9.9; 11.1 9.6 9.5 12.7. 64 rows 16.0 12.3 10.7
+  // 13.7; 11.4 10.3 11.2 20.3. 148 rows 16.8 14.6 20.3 -; 12.7 14.3 24.8 -. 200 rows 18.7 20.4 - -; 17.9 22.1 - -. 1 x
+  // 50000 7.8 7.1 6.2 6.5; 7.5 6.9 6.5 7.2. 32 rows 9.8 8.5 7.4 8.4; 8.1 7.6 7.6 12.0. 200 rows 11.7 13.9 - -; 12.4
+  // 17.1 - -. 148 x 16032 6.5 7.1 12.8 -; 5.9 8.7 19.7 -. 400 rows 8.2; 11.2. k = 5, 1 x 1000 4.3; 4.8.
   const int64_t bytes = static_cast<int64_t>(a.V) * sizeof(T);
-  while (cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * sms && bytes / (cluster * 2) >= 30 * 1024) cluster *= 2;
+  const bool wide = a.rows <= sms && bytes >= 16 * 1024;
+  int cluster = 1;
+  for (int c = 2; wide && c <= kMaxCluster && a.rows * c <= sms; c *= 2) {
+    if (a.V / c < (a.rows * c <= sms / 2 ? 12000 : 24000)) break;
+    cluster = c;
+  }
   cudaLaunchConfig_t cfg{};
   const int64_t grid = a.rows * cluster;
   if (grid > 0x7fffffff) throw std::invalid_argument("token_logprobs: too many rows for one launch");
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(wide ? 512 : 256);
   cfg.stream = s;
-  // Four CTAs fit on an SM; of a grid that fills two to three per SM some SMs would get four and others two. Shared
-  // memory that nobody uses makes it three: 300 x 128256 bf16 30.7 -> 25.2 us. (Clusters have up to two per SM.)
+  // Four CTAs of 256 threads fit on an SM; of a grid that fills two to three per SM some SMs would get four and others
+  // two. Shared memory that nobody uses makes it three: 300 x 128256 bf16 30.7 -> 25.2 us.
   if (grid > 2 * sms && grid <= 3 * sms) cfg.dynamicSmemBytes = kPad;
-  const auto kernel = cluster > 1 ? k_token_logprobs<T, true> : k_token_logprobs<T, false>;
+  const auto kernel = cluster > 1 ? k_token_logprobs<T, true, 512>
+                                  : (wide ? k_token_logprobs<T, false, 512> : k_token_logprobs<T, false, 256>);
   static std::atomic<bool> ready[64];  // by device; setting it twice does no harm
   int dev = 0;
   NAB_CUDA_CHECK(cudaGetDevice(&dev));
   if (cfg.dynamicSmemBytes > 0 && !ready[dev & 63].load(std::memory_order_acquire)) {
-    NAB_CUDA_CHECK(cudaFuncSetAttribute(k_token_logprobs<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPad));
+    NAB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPad));
     ready[dev & 63].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute attrs[2];

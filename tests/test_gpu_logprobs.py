@@ -72,6 +72,23 @@ def test_token_logprobs(rows, v, k, dtype):
     check(logits(rows, v, dtype, rows + v), tokens(rows, v), k)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,v,k", [(149, 30001, 5), (148, 30001, 5), (148, 8191, 32), (75, 47999, 3), (74, 24001, 32),
+                                      (37, 50003, 20), (18, 100003, 32), (18, 96001, 1), (9, 200003, 7), (9, 12001, 0)])
+def test_rows_shared_by_several_ctas_and_not(rows, v, k, dtype):
+    check(logits(rows, v, dtype, rows + v), tokens(rows, v), k)
+
+
+@pytest.mark.parametrize("copies", [6, 20, 60])
+def test_more_large_values_than_are_collected(copies):
+    v = 131072
+    x = logits(2, v, F32, 8, 1.0)
+    i = torch.arange(v, device="cuda")
+    hot = (i % 4096) < 64
+    x[:, hot] = 50 + (i[hot] * 7919 % 2048).float() / 64
+    check(x.repeat(copies, 1), tokens(2 * copies, v), 32)
+
+
 @pytest.mark.parametrize("dtype,offset", [(BF, 1), (BF, 7), (FP, 3), (F32, 1), (F32, 3)])
 def test_rows_of_any_alignment(dtype, offset):
     big = logits(9, 5003 + 20, dtype, 3)
