@@ -216,9 +216,10 @@ class LlamaTPDecoder:
         self.top_k = logprobs
         self.logprobs: TokenLogprobs | None = None
         self.v_start = self.v_local * self.rank
-        self.v_valid = min(self.v_local, cfg.vocab - self.v_start)
-        if logprobs is not None and not 0 <= logprobs <= min(32, self.v_valid):
-            raise ValueError("logprobs must be from 0 to 32 and at most this rank's share of the vocabulary")
+        self.v_valid = min(self.v_local, max(0, cfg.vocab - self.v_start))
+        least = min(self.v_local, cfg.vocab - self.v_local * (self.world - 1))  # the last rank's: refused on all alike
+        if logprobs is not None and (least < 1 or not 0 <= logprobs <= min(32, least)):
+            raise ValueError("logprobs must be from 0 to 32 and at most each rank's share of the vocabulary")
         self._gathered = torch.empty(W * batch * 2, device=self.device, dtype=torch.float32)
 
     # --------------------------------------------------------------- pieces --
@@ -301,9 +302,15 @@ class LlamaTPDecoder:
             if trace is not None:
                 trace.append(self.h.float().clone())
         self._proj(self.x, self._w(-1, "lm_head"), self.logits)
-        val, idx = self.logits.float().max(dim=-1)
+        # columns past the vocabulary pad the last shards' weights: never chosen
+        logits = self.logits[:, :self.v_valid]
+        if self.v_valid > 0:
+            val, idx = logits.float().max(dim=-1)
+            idx = idx + self.v_start
+        else:  # a shard of padding alone: token 0 at -inf
+            val, idx = self.logits.new_full((self.B,), -math.inf, dtype=torch.float32), torch.zeros_like(self.tokens)
         if self.world > 1:
-            mine = torch.stack([val, (idx + self.rank * self.v_local).float()], dim=-1).reshape(-1)
+            mine = torch.stack([val, idx.float()], dim=-1).reshape(-1)
             dist.all_gather_into_tensor(self._gathered, mine)
             allv = self._gathered.view(self.world, self.B, 2)
             best = allv[:, :, 0].argmax(dim=0)
@@ -311,8 +318,7 @@ class LlamaTPDecoder:
         else:
             self.next_tokens.copy_(idx)
         if self.top_k is not None:
-            # columns past the vocabulary pad the last shard's weight
-            r = token_logprobs(self.logits[:, :self.v_valid], self.next_tokens, self.top_k, self.v_start)
+            r = token_logprobs(logits, self.next_tokens, self.top_k, self.v_start)
             self.logprobs = gather_token_logprobs(r) if self.world > 1 else r
         if check_enabled() and not torch.cuda.is_current_stream_capturing():
             check_kernels()
