@@ -342,7 +342,9 @@ void assign_pages(cudaStream_t s, const AssignPagesArgs& a) {
   const int64_t rows = std::max({a.T, a.B, 1});
   const int grid = static_cast<int>(std::min<int64_t>(148, (rows + kAssignThreads - 1) / kAssignThreads));
   const size_t smem = (static_cast<size_t>(a.B) + (a.starts ? a.B + 1 : 0)) * sizeof(int);
-  if (smem > 48 * 1024)  // per device and cheap: set on each such call
+  // The limit of 48 KB without opting in is for this and the kernel's static shared memory together. The attribute is
+  // the device's and cheap: set on each such call.
+  if (smem > 32 * 1024)
     NAB_CUDA_CHECK(cudaFuncSetAttribute(k_assign_pages, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (2 * kMaxPagedRequests + 1) * static_cast<int>(sizeof(int))));
   launch(k_assign_pages, grid, kAssignThreads, smem, s, "assign_pages", a);
