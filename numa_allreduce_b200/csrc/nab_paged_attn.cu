@@ -236,8 +236,9 @@ __global__ void __launch_bounds__(kPThreads, 2)
     const int segment = static_cast<int>(blockIdx.x) / a.cluster, rank = static_cast<int>(blockIdx.x) % a.cluster;
     w.b = segment / HH;
     w.h = segment % HH;
-    // loaded beside the length, which says only then which of them count
-    if (warp == kWarps && lane < a.M) early = __ldg(a.tables + w.b * a.table_stride + lane);
+    // loaded beside the length, which says only then which of them count (plain loads of the table: the launch before
+    // may have written it while this CTA was already resident)
+    if (warp == kWarps && lane < a.M) early = a.tables[w.b * a.table_stride + lane];
     const int raw = a.lengths[w.b];
     if (tid == 0 && rank == 0 && w.h == 0 && (raw < 0 || raw > static_cast<int64_t>(a.M) * a.P))
       record_local_failure(a.err, a.err_host, kErrBadLaunch, kStageBounds, static_cast<uint32_t>(w.b));
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kPThreads, 2)
     // comes to w.b so that the next request starts without a wait
     int window = 0, ids = 0, ahead = 0;
     auto load_ids = [&](int b, int first) {
-      return b < a.B && first + lane < a.M ? __ldg(a.tables + b * a.table_stride + first + lane) : 0;
+      return b < a.B && first + lane < a.M ? a.tables[b * a.table_stride + first + lane] : 0;
     };
     bool more = w.x < w.x1, given_up = false;
     if (more) {

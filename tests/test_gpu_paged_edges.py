@@ -7,6 +7,10 @@ import subprocess
 import sys
 
 import pytest
+import torch
+
+import numa_allreduce_b200 as nab
+from test_gpu_paged import BF, check_attention, clean_record, gen  # noqa: F401 (clean_record: for every test)
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +35,49 @@ for b in [int(x) for x in sys.argv[1:]]:
     for counts in (["6135", "6136"], ["6140"], ["6143", "6144", "6145"], ["8192"]):
         p = subprocess.run([sys.executable, "-c", script, *counts], cwd=root, capture_output=True, text=True, timeout=300)
         assert p.returncode == 0, p.stderr[-2000:]
+
+
+# ---------------------------------------------------------- paged_attention --
+@pytest.mark.parametrize("batch,cached,page", [(2, 900, 16), (100, 1500, 16), (300, 100, 32)])  # cluster, even, whole
+def test_attention_directly_after_assign_pages(batch, cached, page):
+    """The table's entries that the launch before has just written, with ids of other pages in their place before."""
+    hq, hkv, d = 8, 1, 128
+    held, new = -(-cached // page), 2 * page
+    width = held + 3
+    pages = batch * width
+    k = torch.randn(pages, hkv, page, d, generator=gen(1), device="cuda").to(BF)
+    v = torch.randn(pages, hkv, page, d, generator=gen(2), device="cuda").to(BF)
+    q = torch.randn(batch, hq, d, generator=gen(3), device="cuda").to(BF)
+    order = torch.randperm(pages, generator=gen(4), device="cuda").int()
+    tables = torch.empty(batch, width, dtype=torch.int32, device="cuda")
+    free = order[batch * held:].contiguous()
+    n = torch.full((batch,), cached, dtype=torch.int32, device="cuda")
+    taken = torch.zeros(1, dtype=torch.int32, device="cuda")
+    starts = torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new
+
+    def steps():
+        outs = []
+        for i in range(6):
+            tables.copy_(stale[i])
+            step = nab.assign_pages(n, tables, free, taken, page, query_start=starts, num_tokens=batch * new)
+            outs.append(nab.paged_attention(q, k, v, tables, step.lengths))
+        return outs, step.lengths
+
+    first = order[:batch * held].view(batch, held)
+    stale = [torch.cat([first, torch.randint(pages, (batch, 3), generator=gen(5 + i), device="cuda").int()], 1)
+             for i in range(6)]
+    steps()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs, lengths = steps()
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert lengths.tolist() == [cached + new] * batch
+    used = -(-(cached + new) // page) - held
+    assert torch.equal(tables[:, held:held + used], free[:batch * used].view(batch, used))
+    for out in outs:
+        check_attention(out, q, k, v, tables, [cached + new] * batch, d ** -0.5)
+    nab.check_kernels()
+    del graph
