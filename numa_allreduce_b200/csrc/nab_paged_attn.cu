@@ -649,6 +649,7 @@ __global__ void __launch_bounds__(kPThreads, 2)
           bar_compute();
           if (warp < 2) take(r, warp);
         }
+        __syncwarp();  // warp 1 overwrites the (max, sum) that its lanes have just read
         if (warp == 1) give(r, 1);
         bar_compute();
         if (warp == 0) take(r, 1);

@@ -2,6 +2,7 @@
 variants and orders of calls that the sizes of an ordinary batch do not reach.
 Oracles and tolerances are those of test_gpu_paged.py."""
 
+import math
 import os
 import subprocess
 import sys
@@ -10,7 +11,7 @@ import pytest
 import torch
 
 import numa_allreduce_b200 as nab
-from test_gpu_paged import BF, check_attention, clean_record, gen  # noqa: F401 (clean_record: for every test)
+from test_gpu_paged import BF, FP, check_attention, clean_record, gen, make_cache  # noqa: F401 (clean_record: for every test)
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,45 @@ def test_attention_directly_after_assign_pages(batch, cached, page):
         check_attention(out, q, k, v, tables, [cached + new] * batch, d ** -0.5)
     nab.check_kernels()
     del graph
+
+
+def repeated(lengths, hq, hkv, d, page, dtype, width, seed):
+    """Checked against the oracle, and the same bits ten times over."""
+    k, v, tables = make_cache(lengths, hkv, d, page, dtype, seed=seed, width=width)
+    q = torch.randn(len(lengths), hq, d, generator=gen(seed), device="cuda").to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = nab.paged_attention(q, k, v, tables, n)
+    check_attention(out, q, k, v, tables, lengths, 1 / math.sqrt(d))
+    for _ in range(10):
+        assert torch.equal(nab.paged_attention(q, k, v, tables, n), out)
+    nab.check_kernels()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page,width", [
+    # even form, few segments cut over many CTAs: one head tile of 9, 12 or 16, two of 9 and 8, three of 14, 13 and 13
+    ([2050], 9, 1, 128, 16, None),
+    ([3100, 1, 900], 12, 1, 128, 16, None),
+    ([8100, 300], 16, 1, 64, 128, None),
+    ([6300, 0, 65], 17, 1, 64, 16, None),
+    ([9000, 20, 4000, 0, 8999], 32, 2, 128, 48, None),
+    # even form, more segments than CTAs
+    ([700 + 9 * i for i in range(60)], 40, 2, 128, 64, None),
+    ([(97 * i) % 401 for i in range(160)], 24, 2, 128, 16, None),
+    ([(97 * i) % 401 for i in range(160)], 8, 2, 128, 16, None),
+    # even form, a table far wider than any request: idle CTAs, requests within one CTA
+    ([130, 0, 5, 64], 12, 1, 128, 16, 8192),
+    ([3000, 0, 5], 8, 2, 64, 64, 2048),
+    ([(31 * i) % 500 for i in range(90)], 32, 2, 128, 32, 4096),
+    ([1], 8, 1, 128, 16, 1000),
+    ([0, 0], 8, 1, 128, 16, 1000),
+    # whole segments
+    ([(37 * i) % 65 for i in range(300)], 32, 2, 128, 16, None),
+    ([(53 * i) % 193 for i in range(200)], 24, 1, 64, 16, None),
+    ([(29 * i) % 48 for i in range(400)], 20, 1, 128, 16, None),
+    # up to 8 heads in the even and whole forms
+    ([5000, 3, 0, 2999], 8, 2, 128, 64, None),
+    ([(41 * i) % 129 for i in range(300)], 8, 1, 128, 128, None),
+])
+def test_every_form_with_few_and_many_heads(lengths, hq, hkv, d, page, width, dtype):
+    repeated(lengths, hq, hkv, d, page, dtype, width, seed=len(lengths) + hq)
