@@ -168,6 +168,18 @@ NAB_DINLINE float ex2(float x) {
   return y;
 }
 
+// The probabilities relative to the maximum are held times 2^kBits, in sums and outputs alike, so it cancels. In fp16
+// one below 2^-25 would be zero and one below 2^-14 lose bits, which in a long cache are many: with 2^15 (its largest
+// is 65504) these become 2^-40 and 2^-29. bf16 has fp32's exponents.
+template <typename T>
+struct ProbShift {
+  static constexpr float kBits = 0.f;
+};
+template <>
+struct ProbShift<__half> {
+  static constexpr float kBits = 15.f;
+};
+
 NAB_DINLINE int64_t min64(int64_t x, int64_t y) { return x < y ? x : y; }
 
 NAB_DINLINE void bar_compute() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
@@ -512,10 +524,11 @@ __global__ void __launch_bounds__(kPThreads, 2)
       const float ms = mn == -INFINITY ? 0.f : mn;
       alpha[r] = ex2(m[r] - ms);
       m[r] = mn;
+      const float base_exp = ms - ProbShift<T>::kBits;
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4 * kSteps; ++e) {
-        v[e] = ex2(v[e] - ms);
+        v[e] = ex2(v[e] - base_exp);
         sum += v[e];
       }
       l[r] = l[r] * alpha[r] + sum;

@@ -124,3 +124,27 @@ def repeated(lengths, hq, hkv, d, page, dtype, width, seed):
 ])
 def test_every_form_with_few_and_many_heads(lengths, hq, hkv, d, page, width, dtype):
     repeated(lengths, hq, hkv, d, page, dtype, width, seed=len(lengths) + hq)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("batch,n,d,group", [(1, 131071, 64, 8), (40, 16383, 128, 4), (40, 16383, 64, 12)])
+@pytest.mark.parametrize("bits", [14, 20, 26, 28])
+def test_many_small_probabilities(batch, n, d, group, bits, dtype):
+    """Eight early positions outweigh each of the others by 2^bits and add nothing to the output: the others are all
+    of it. (Eight, 16 apart: one for every warp. 40 requests of 8 kv heads, with the same pages: each in few CTAs.)"""
+    page, hkv, top = 64, 8, 8
+    k, v, tables = make_cache([n], hkv, d, page, dtype, seed=bits)
+    k[:], v[:] = 0, 1024  # (rows past the length too)
+    for i in range(top):
+        at = tables[0, 16 * i // page].item()
+        k[at, :, 16 * i % page + 3], v[at, :, 16 * i % page + 3] = 1, 0  # scores: d there, 0 elsewhere, exact
+    q = torch.ones(batch, hkv * group, d, device="cuda", dtype=dtype)
+    scale = bits * math.log(2) / d
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = nab.paged_attention(q, k, v, tables.expand(batch, -1), lengths, scale=scale)
+    want = 1024 * (n - top) / (n - top + top * math.exp(d * torch.tensor(scale, dtype=torch.float32).item()))
+    # the probabilities' and the output's rounding; scores, exponentials and sums as in check_attention with exact scores
+    # (an exponent of up to 28 with four roundings of 2^-24, an exp2 of 2^-22, for the weight and for the sum)
+    u = torch.finfo(dtype).eps / 2
+    tol = want * (2 * u + 2 * (28 * 4 * 2 ** -24 + 2 ** -22) + (n / 64 + 64) * 2 ** -22) + torch.finfo(dtype).tiny
+    assert (out.double() - want).abs().max().item() <= tol
