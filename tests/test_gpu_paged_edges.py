@@ -11,7 +11,8 @@ import pytest
 import torch
 
 import numa_allreduce_b200 as nab
-from test_gpu_paged import BF, FP, check_attention, clean_record, gen, make_cache  # noqa: F401 (clean_record: for every test)
+from test_gpu_paged import BF, FP, attention_oracle, check_attention, gen, make_cache
+from test_gpu_paged import clean_record  # noqa: F401 (for every test)
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +149,58 @@ def test_many_small_probabilities(batch, n, d, group, bits, dtype):
     u = torch.finfo(dtype).eps / 2
     tol = want * (2 * u + 2 * (28 * 4 * 2 ** -24 + 2 ** -22) + (n / 64 + 64) * 2 ** -22) + torch.finfo(dtype).tiny
     assert (out.double() - want).abs().max().item() <= tol
+
+
+def exact_scores(lengths, hq, hkv, d, page, dtype, seed):
+    """A cache and queries whose scores are sums of whole numbers: exact whatever the order."""
+    k, v, tables = make_cache(lengths, hkv, d, page, dtype, seed=seed)
+    k.copy_(torch.where(k.isnan(), k, (k * 1.5).round().clamp(-2, 2)))
+    q = torch.randint(-2, 3, (len(lengths), hq, d), generator=gen(seed), device="cuda").to(dtype)
+    return q, k, v, tables
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page", [
+    ([3, 5, 17, 64, 200], 8, 2, 128, 16),          # clusters
+    ([3, 5, 17, 64, 200], 12, 1, 128, 16),
+    ([3, 40, 17, 64, 300], 16, 2, 64, 32),
+    ([2100, 3, 900], 4, 1, 128, 16),               # even
+    ([2100, 3, 900], 16, 1, 128, 16),
+    ([4100, 50, 900], 40, 2, 64, 128),
+    ([(37 * i) % 65 for i in range(300)], 8, 1, 128, 16),  # whole
+    ([(37 * i) % 65 for i in range(300)], 9, 1, 128, 16),
+])
+def test_no_rounding_but_the_outputs(lengths, hq, hkv, d, page, dtype):
+    """Within the rounding of the output and fp32 work, where the terms cancel too.
+
+    Scores are exact. Their product with scale * log2(e), itself rounded twice, and the difference to the maximum are
+    off by 4 V 2^-24 for exponents up to V, exp2 by 2^-22: a weight by 4 V 2^-24 + 2^-22 (ln 2 < 1), and the sum of
+    them as much. A probability is held in two 16-bit values, off by u^2; the sums over n positions are as in
+    check_attention.
+    """
+    scale = 0.02
+    q, k, v, tables = exact_scores(lengths, hq, hkv, d, page, dtype, seed=len(lengths) + hq)
+    out = nab.paged_attention(q, k, v, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda"), scale=scale)
+    scale = torch.tensor(scale, dtype=torch.float32).item()
+    want, A, qk = attention_oracle(q, k, v, tables, lengths, scale)
+    n = torch.tensor(lengths, device="cuda", dtype=torch.float64)[:, None, None]
+    u, V = torch.finfo(dtype).eps / 2, 1.4427 * scale * 2 * qk
+    own = 2 * (4 * V * 2 ** -24 + 2 ** -22) + u * u + (n / 64 + 64) * 2 ** -22
+    tol = u * want.abs() + own * A + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item()} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("length,hq", [(100, 8), (100, 12), (5000, 4), (5000, 16)])
+def test_infinite_values_stay_infinite(length, hq, dtype):
+    """An infinity of v is the output's in its dim; the other dims are as ever."""
+    q, k, v, tables = exact_scores([length], hq, 1, 128, 16, dtype, seed=3)
+    v[tables[0, 2].item(), 0, 7, 5] = math.inf
+    v[tables[0, 4].item(), 0, 1, 9] = -math.inf
+    out = nab.paged_attention(q, k, v, tables, torch.tensor([length], dtype=torch.int32, device="cuda"), scale=0.02)
+    assert (out[..., 5] == math.inf).all() and (out[..., 9] == -math.inf).all()
+    finite = [i for i in range(128) if i not in (5, 9)]
+    v[tables[0, 2].item(), 0, 7, 5] = v[tables[0, 4].item(), 0, 1, 9] = 0
+    want = nab.paged_attention(q, k, v, tables, torch.tensor([length], dtype=torch.int32, device="cuda"), scale=0.02)
+    assert torch.equal(out[..., finite], want[..., finite])
