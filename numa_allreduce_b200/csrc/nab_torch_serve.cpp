@@ -7,12 +7,12 @@
 // in place of a look into os.environ, 0.6 us).
 //
 // Every argument is checked here before anything is launched. A bad one is
-// refused with its name whatever device it lies on; tensors on a device other
-// than CUDA are refused last, and so is one that requires a gradient. The GIL
-// is released during the call.
+// refused with its name whatever device it lies on, and so are tensors that
+// share memory with one that the call writes; tensors on a device other than
+// CUDA are refused last, and so is one that requires a gradient. The GIL is
+// released during the call.
 #include <Python.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/record_function.h>
@@ -50,6 +50,49 @@ void check_devices(const char* op, std::initializer_list<Named> tensors) {
   }
 }
 
+// The bytes of a tensor whose first dimension may have its rows apart and whose other ones are contiguous.
+struct Extent {
+  const char* name;
+  uintptr_t at = 0;
+  int64_t rows = 0, width = 0, step = 0;  // bytes but for `rows`
+  Extent(const char* n, const at::Tensor* t) : name(n) {
+    if (t == nullptr || t->numel() == 0) return;
+    at = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    const int64_t e = t->element_size();
+    if (t->is_contiguous()) {
+      rows = 1;
+      width = t->numel() * e;
+    } else {
+      rows = t->size(0);
+      width = t->numel() / rows * e;
+      step = t->stride(0) * e;
+    }
+  }
+};
+
+// Whether a row of `a` shares bytes with `b`, which is one block.
+bool touches(const Extent& a, const Extent& b) {
+  if (a.at == 0 || b.at == 0) return false;
+  const int64_t lo = static_cast<int64_t>(b.at - a.at), hi = lo + b.width;  // b's bytes, counted from a's first
+  if (a.step == 0) return lo < a.width && hi > 0;
+  // the first row that ends behind b's first byte
+  const int64_t r = lo < a.width ? 0 : (lo - a.width) / a.step + 1;
+  return r < a.rows && r * a.step < hi;
+}
+
+// No tensor that the call writes shares memory with another one of the call. Of two tensors with rows apart only one
+// may be given here as written.
+void check_apart(const char* op, std::initializer_list<Extent> written, std::initializer_list<Extent> read) {
+  const auto check = [op](const Extent& w, const Extent& r) {
+    TORCH_CHECK(!(w.rows > 1 ? touches(w, r) : touches(r, w)), op, ": ", w.name, " and ", r.name,
+                " overlap in memory");
+  };
+  for (const Extent* w = written.begin(); w != written.end(); ++w) {
+    for (const Extent* v = w + 1; v != written.end(); ++v) check(*w, *v);
+    for (const Extent& r : read) check(*w, r);
+  }
+}
+
 void check_vector(const char* op, const char* name, const at::Tensor& t, at::ScalarType type, int64_t n) {
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.scalar_type() == type, op, ": ", name,
               " must be a contiguous ", type, " tensor of ", n, " elements");
@@ -73,7 +116,7 @@ void check_pages(const char* op, const at::Tensor& k, const at::Tensor& v, at::S
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, op, ": head_dim must be 64 or 128, got ", k.size(3));
   TORCH_CHECK(k.size(0) * k.size(1) * k.size(2) < INT_MAX, op, ": too many page rows");
   TORCH_CHECK(aligned16(k) && aligned16(v), op, ": k_pages and v_pages must be 16-byte aligned");
-  if (k.is_cuda()) at::assert_no_overlap(k, v);
+  check_apart(op, {{"k_pages", &k}}, {{"v_pages", &v}});
 }
 
 // An uninitialised tensor on the device of `like` (the call's device guard is set): the allocator without the
@@ -141,13 +184,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
               ": page_size must be a multiple of 16, got ", page_size);
   TORCH_CHECK(num_tokens >= 0 && num_tokens <= (1 << 30), op, ": bad num_tokens ", num_tokens);
   TORCH_CHECK(query_start || num_tokens >= B, op, ": num_tokens must be at least the ", B, " requests");
+  const at::Tensor* starts = query_start ? &*query_start : nullptr;
+  check_apart(op, {{"block_tables", &block_tables}},
+              {{"cached", &cached}, {"query_start", starts}, {"free_pages", &free_pages}, {"taken", &taken}});
   check_devices(op, {{"cached", &cached},
-                     {"query_start", query_start ? &*query_start : nullptr},
+                     {"query_start", starts},
                      {"block_tables", &block_tables},
                      {"free_pages", &free_pages},
                      {"taken", &taken}});
-  for (const at::Tensor* t : {&cached, &free_pages, &taken}) at::assert_no_overlap(block_tables, *t);
-  if (query_start) at::assert_no_overlap(block_tables, *query_start);
   const at::cuda::CUDAGuard guard(cached.device());
   Outputs outputs(cached);
   outputs.add({num_tokens}, at::kInt);
@@ -158,7 +202,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
   at::Tensor positions = outputs[0], slots = outputs[1], lengths = outputs[2], taken_out = outputs[3];
   nab::AssignPagesArgs a{};
   a.cached = cached.const_data_ptr<int>();
-  a.starts = query_start ? query_start->const_data_ptr<int>() : nullptr;
+  a.starts = starts ? starts->const_data_ptr<int>() : nullptr;
   a.tables = block_tables.mutable_data_ptr<int>();
   a.table_stride = B == 1 ? 0 : block_tables.stride(0);
   a.free_pages = free_pages.const_data_ptr<int>();
@@ -208,6 +252,15 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
     check_vector(op, name, **w, qkv.scalar_type(), D);
     TORCH_CHECK(aligned16(**w), op, ": ", name, " must be 16-byte aligned");
   }
+  const at::Tensor *qw = q_norm ? &*q_norm : nullptr, *kw = k_norm ? &*k_norm : nullptr;
+  check_apart(op, {{"k_pages", &k_pages}, {"v_pages", &v_pages}, {"out", given}},
+              {{"qkv", &qkv},
+               {"cos", &cos},
+               {"sin", &sin},
+               {"positions", &positions},
+               {"slots", &slots},
+               {"q_norm", qw},
+               {"k_norm", kw}});
   check_devices(op, {{"qkv", &qkv},
                      {"cos", &cos},
                      {"sin", &sin},
@@ -215,14 +268,9 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
                      {"slots", &slots},
                      {"k_pages", &k_pages},
                      {"v_pages", &v_pages},
-                     {"q_norm", q_norm ? &*q_norm : nullptr},
-                     {"k_norm", k_norm ? &*k_norm : nullptr},
+                     {"q_norm", qw},
+                     {"k_norm", kw},
                      {"out", given}});
-  for (const at::Tensor* t : {&k_pages, &v_pages}) {
-    at::assert_no_overlap(*t, qkv);
-    if (given) at::assert_no_overlap(*given, *t);
-  }
-  if (given) at::assert_no_overlap(*given, qkv);
   const at::cuda::CUDAGuard guard(qkv.device());
   at::Tensor out = given ? *given : fresh({T, Hq, D}, qkv.scalar_type(), qkv);
   nab::RopeAppendArgs a{};
@@ -232,8 +280,8 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
   a.sin_t = sin.const_data_ptr<float>();
   a.positions = positions.const_data_ptr<int>();
   a.slots = slots.const_data_ptr<int64_t>();
-  a.q_norm = q_norm ? q_norm->const_data_ptr() : nullptr;
-  a.k_norm = k_norm ? k_norm->const_data_ptr() : nullptr;
+  a.q_norm = qw ? qw->const_data_ptr() : nullptr;
+  a.k_norm = kw ? kw->const_data_ptr() : nullptr;
   a.q_out = out.mutable_data_ptr();
   a.k_pages = k_pages.mutable_data_ptr();
   a.v_pages = v_pages.mutable_data_ptr();
@@ -271,15 +319,18 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
               op, ": block_tables must be int32 [", B, ", pages] with contiguous rows");
   TORCH_CHECK(block_tables.size(1) * P < INT_MAX, op, ": block_tables is too wide");
   check_vector(op, "lengths", lengths, at::kInt, B);
+  check_apart(op, {{"out", given}},
+              {{"q", &q},
+               {"k_pages", &k_pages},
+               {"v_pages", &v_pages},
+               {"block_tables", &block_tables},
+               {"lengths", &lengths}});
   check_devices(op, {{"q", &q},
                      {"k_pages", &k_pages},
                      {"v_pages", &v_pages},
                      {"block_tables", &block_tables},
                      {"lengths", &lengths},
                      {"out", given}});
-  if (given) {
-    for (const at::Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(*given, *t);
-  }
   const at::cuda::CUDAGuard guard(q.device());
   at::Tensor out = given ? *given : fresh({B, Hq, D}, q.scalar_type(), q);
   if (B == 0) return out;

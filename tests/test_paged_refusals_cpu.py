@@ -1,0 +1,109 @@
+"""Calls of the paged-cache operators and the token log-probabilities that must
+be refused before anything is launched: tensors that share memory with one
+that the call writes."""
+
+import pytest
+import torch
+
+import numa_allreduce_b200 as nab
+
+BF = torch.bfloat16
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def as_type(raw, dtype, offset, *shape):
+    """A tensor in the bytes of `raw` from `offset` on."""
+    n = torch.Size(shape).numel() * dtype.itemsize
+    return raw.view(-1).view(torch.uint8)[offset:offset + n].view(dtype).view(shape)
+
+
+def append(**kw):
+    a = dict(qkv=torch.zeros(3, 8 * 64, dtype=BF), cos=torch.zeros(10, 32), sin=torch.zeros(10, 32),
+             positions=i32(3), slots=torch.arange(3), k_pages=torch.zeros(2, 2, 16, 64, dtype=BF),
+             v_pages=torch.zeros(2, 2, 16, 64, dtype=BF), q_heads=4)
+    a.update(kw)
+    return nab.rope_append_paged(**a)
+
+
+def attend(**kw):
+    a = dict(q=torch.zeros(2, 4, 64, dtype=BF), k_pages=torch.zeros(3, 2, 16, 64, dtype=BF),
+             v_pages=torch.zeros(3, 2, 16, 64, dtype=BF), block_tables=i32(2, 3), lengths=i32(2))
+    a.update(kw)
+    return nab.paged_attention(**a)
+
+
+def assign(**kw):
+    a = dict(cached=i32(2), block_tables=i32(2, 4), free_pages=i32(3), taken=i32(1), page_size=16)
+    a.update(kw)
+    return nab.assign_pages(**a)
+
+
+def refused(call, match="overlap"):
+    with pytest.raises(RuntimeError, match=match):
+        call()
+
+
+# --------------------------------------------------------- shared memory --
+def test_append_does_not_write_what_it_reads():
+    pool = torch.zeros(1 << 15, dtype=BF)
+    pages = pool[:4096].view(2, 2, 16, 64)
+    for name in ("k_pages", "v_pages"):
+        kw = {name: pages}
+        refused(lambda: append(qkv=pool[1024:1024 + 1536].view(3, 512), **kw))
+        refused(lambda: append(cos=as_type(pool, torch.float32, 4096, 10, 32), **kw))
+        refused(lambda: append(sin=as_type(pool, torch.float32, 0, 10, 32), **kw))
+        refused(lambda: append(positions=as_type(pool, torch.int32, 8188, 3), **kw))
+        refused(lambda: append(slots=as_type(pool, torch.int64, 64, 3), **kw))
+        refused(lambda: append(q_norm=pool[64:128], **kw))
+        refused(lambda: append(k_norm=pool[4032:4096], **kw))
+        refused(lambda: append(out=pool[3840:3840 + 768].view(3, 4, 64), **kw))
+        # right behind the pages: not refused for that
+        refused(lambda: append(qkv=pool[4096:4096 + 1536].view(3, 512), out=pool[8192:8192 + 768].view(3, 4, 64), **kw),
+                "must be a CUDA tensor")
+    refused(lambda: append(k_pages=pages, v_pages=pool[2048:2048 + 4096].view(2, 2, 16, 64)))
+    out = pool[8192:8192 + 768].view(3, 4, 64)
+    refused(lambda: append(out=out, qkv=pool[8192:8192 + 1536].view(3, 512)))
+    refused(lambda: append(out=out, slots=as_type(pool, torch.int64, 2 * 8192, 3)))
+
+
+def test_append_with_rows_apart():
+    """Rows of qkv further apart than their width: what lies between them is free for other tensors."""
+    wide = torch.zeros(3, 4096, dtype=BF)
+    qkv = wide[:, 1024:1024 + 512]
+    flat = wide.view(-1)
+    refused(lambda: append(qkv=qkv, out=flat[4096 + 1024 + 504:][:768].view(3, 4, 64)))  # the end of the second row
+    refused(lambda: append(qkv=qkv, out=flat[2 * 4096 + 512:][:768].view(3, 4, 64)))     # up to the third row's start
+    refused(lambda: append(qkv=qkv, k_pages=flat[:4096].view(2, 2, 16, 64)))
+    refused(lambda: append(qkv=qkv, out=flat[2048:][:768].view(3, 4, 64)), "must be a CUDA tensor")
+    refused(lambda: append(qkv=qkv, out=flat[4096 + 256:][:768].view(3, 4, 64)), "must be a CUDA tensor")
+    refused(lambda: append(qkv=qkv, out=flat[8192 + 1536:][:768].view(3, 4, 64)), "must be a CUDA tensor")
+
+
+def test_attention_does_not_write_what_it_reads():
+    pool = torch.zeros(1 << 14, dtype=BF)
+    out = pool[1024:1536].view(2, 4, 64)
+    refused(lambda: attend(out=out, q=pool[1024:1536].view(2, 4, 64)))
+    wide = torch.zeros(2, 1024, dtype=BF)
+    refused(lambda: attend(q=wide[:, :256].view(2, 4, 64), out=wide.view(-1)[768:1280].view(2, 4, 64)))
+    refused(lambda: attend(q=wide[:, :256].view(2, 4, 64), out=wide.view(-1)[256:768].view(2, 4, 64)),
+            "must be a CUDA tensor")
+    refused(lambda: attend(out=out, k_pages=pool[:6144].view(3, 2, 16, 64)))
+    refused(lambda: attend(out=out, v_pages=pool[1528:][:6144].view(3, 2, 16, 64)))
+    refused(lambda: attend(out=out, block_tables=as_type(pool, torch.int32, 2048, 2, 3)))
+    refused(lambda: attend(out=out, lengths=as_type(pool, torch.int32, 3064, 2)))
+
+
+def test_assign_pages_does_not_write_what_it_reads():
+    wide = i32(2, 16)
+    flat = wide.view(-1)
+    tables = wide[:, 4:8]
+    refused(lambda: assign(block_tables=tables, cached=flat[20:22]))
+    refused(lambda: assign(block_tables=tables, taken=flat[7:8]))
+    refused(lambda: assign(block_tables=tables, free_pages=flat[1:5]))
+    refused(lambda: assign(block_tables=tables, query_start=flat[18:21], num_tokens=2))
+    # between the rows of the table
+    refused(lambda: assign(block_tables=tables, cached=flat[0:2], taken=flat[3:4], free_pages=flat[8:20],
+                           query_start=flat[24:27], num_tokens=2), "must be a CUDA tensor")
