@@ -9,8 +9,9 @@
 // Every argument is checked here before anything is launched. A bad one is
 // refused with its name whatever device it lies on, and so are tensors that
 // share memory with one that the call writes; tensors on a device other than
-// CUDA are refused last, and so is one that requires a gradient. The GIL is
-// released during the call.
+// CUDA are refused last, and so is one that asks for a derivative. There is no
+// dispatcher to take a fake, batched or wrapped tensor elsewhere: these are
+// refused. The GIL is released during the call.
 #include <Python.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -37,13 +38,18 @@ namespace {
 using OptTensor = std::optional<at::Tensor>;
 using Named = std::pair<const char*, const at::Tensor*>;
 
-// The last check of every op: one CUDA device for all, and no gradients asked for.
+// The last check of every op: no derivative asked for, and one CUDA device for all.
 void check_devices(const char* op, std::initializer_list<Named> tensors) {
   const at::Tensor& first = *tensors.begin()->second;
   for (const auto& [name, t] : tensors) {
     if (t == nullptr) continue;
     TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), op, ": ", name,
                 " requires a gradient; this operator has none (use torch.no_grad())");
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, ": ", name,
+                " carries a forward-mode tangent; this operator has no derivative");
+  }
+  for (const auto& [name, t] : tensors) {
+    if (t == nullptr) continue;
     TORCH_CHECK(t->is_cuda(), op, ": ", name, " must be a CUDA tensor");
     TORCH_CHECK(t->device() == first.device(), op, ": ", name, " is on ", t->device(), ", ", tensors.begin()->first,
                 " on ", first.device());
@@ -407,6 +413,15 @@ LogprobsResult token_logprobs(const at::Tensor& logits, const at::Tensor& tokens
 }
 
 // ------------------------------------------------------ Python side --
+// Whether the tensor's bytes are its values: not a fake, traced, batched or wrapped one, which the dispatcher would have
+// taken elsewhere, nor one with a negation or conjugation pending.
+bool plain(const at::Tensor& t) {
+  using K = c10::DispatchKey;
+  constexpr c10::DispatchKeySet other({K::Python, K::Functionalize, K::FuncTorchBatched, K::FuncTorchGradWrapper,
+                                       K::BatchedNestedTensor, K::Negative, K::Conjugate, K::ZeroTensor});
+  return !t.key_set().has_any(other) && t.layout() == at::kStrided && !t.is_meta() && t.has_storage();
+}
+
 // The positional arguments of a call, taken one after the other.
 class Args {
  public:
@@ -416,7 +431,10 @@ class Args {
   const at::Tensor& tensor(const char* name) {
     PyObject* o = args_[i_++];
     TORCH_CHECK_TYPE(THPVariable_Check(o), op_, ": ", name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK(t.defined() && plain(t), op_, ": ", name, " must be a plain tensor, got ", Py_TYPE(o)->tp_name, " of ",
+                t.layout(), " layout, keys ", t.key_set());
+    return t;
   }
   OptTensor optional_tensor(const char* name) {
     if (args_[i_] == Py_None) {

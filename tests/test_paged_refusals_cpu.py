@@ -107,3 +107,55 @@ def test_assign_pages_does_not_write_what_it_reads():
     # between the rows of the table
     refused(lambda: assign(block_tables=tables, cached=flat[0:2], taken=flat[3:4], free_pages=flat[8:20],
                            query_start=flat[24:27], num_tokens=2), "must be a CUDA tensor")
+
+
+# ------------------------------------------ tensors that are not plain memory --
+def logprobs(**kw):
+    a = dict(logits=torch.zeros(2, 10), tokens=torch.zeros(2, dtype=torch.int64), top_k=3)
+    a.update(kw)
+    return nab.token_logprobs(**a)
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    with fw.dual_level():
+        def dual(*shape, dtype=BF):
+            return fw.make_dual(torch.zeros(*shape, dtype=dtype), torch.ones(*shape, dtype=dtype))
+
+        refused(lambda: logprobs(logits=dual(2, 10, dtype=torch.float32)), "logits.*tangent")
+        refused(lambda: append(qkv=dual(3, 512)), "qkv.*tangent")
+        refused(lambda: append(k_norm=dual(64)), "k_norm.*tangent")
+        refused(lambda: append(k_pages=dual(2, 2, 16, 64)), "k_pages.*tangent")
+        refused(lambda: attend(q=dual(2, 4, 64)), "q .*tangent")
+        refused(lambda: attend(v_pages=dual(3, 2, 16, 64)), "v_pages.*tangent")
+        refused(lambda: attend(out=dual(2, 4, 64)), "out.*tangent")
+        with torch.no_grad():
+            refused(lambda: attend(q=dual(2, 4, 64)), "q .*tangent")
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        fake = torch.empty(2, 10, device="cuda"), torch.empty(2, 4, 64, dtype=BF, device="cuda")
+    refused(lambda: logprobs(logits=fake[0]), "logits must be a plain tensor")
+    refused(lambda: attend(q=fake[1]), "q must be a plain tensor")
+    refused(lambda: attend(out=fake[1]), "out must be a plain tensor")
+    refused(lambda: logprobs(logits=torch.zeros(2, 10, device="meta")), "logits must be a plain tensor")
+    refused(lambda: logprobs(logits=torch.zeros(2, 10).to_sparse()), "logits must be a plain tensor")
+    refused(lambda: logprobs(logits=torch._neg_view(torch.zeros(2, 10))), "logits must be a plain tensor")
+    refused(lambda: logprobs(logits=torch._efficientzerotensor(2, 10)), "logits must be a plain tensor")
+    refused(lambda: torch.vmap(lambda x: logprobs(logits=x).logprob)(torch.zeros(4, 2, 10)), "plain tensor")
+    refused(lambda: torch.func.jvp(lambda x: logprobs(logits=x).logprob, (torch.zeros(2, 10),), (torch.ones(2, 10),)),
+            "plain tensor|tangent")
+    refused(lambda: torch.func.functionalize(lambda x: logprobs(logits=x).logprob)(torch.zeros(2, 10)), "plain tensor")
+
+    class Wrapped(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    refused(lambda: logprobs(logits=torch.zeros(2, 10).as_subclass(Wrapped)), "logits must be a plain tensor")
+    refused(lambda: logprobs(logits=torch.nn.Parameter(torch.zeros(2, 10), requires_grad=False)),
+            "must be a CUDA tensor")  # a parameter is one
