@@ -323,7 +323,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == B && block_tables.scalar_type() == at::kInt &&
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
               op, ": block_tables must be int32 [", B, ", pages] with contiguous rows");
-  TORCH_CHECK(block_tables.size(1) * P < INT_MAX, op, ": block_tables is too wide");
+  TORCH_CHECK(block_tables.size(1) * P <= INT_MAX - 127, op, ": block_tables is too wide");  // and a tile fits 32 bits
   check_vector(op, "lengths", lengths, at::kInt, B);
   check_apart(op, {{"out", given}},
               {{"q", &q},

@@ -159,3 +159,11 @@ def test_tensors_without_memory_of_their_own_are_refused():
     refused(lambda: logprobs(logits=torch.zeros(2, 10).as_subclass(Wrapped)), "logits must be a plain tensor")
     refused(lambda: logprobs(logits=torch.nn.Parameter(torch.zeros(2, 10), requires_grad=False)),
             "must be a CUDA tensor")  # a parameter is one
+
+
+# ------------------------------------------------------------------ sizes --
+def test_a_table_for_more_positions_than_fit_32_bits():
+    """The tiles of a request are counted from its length and a tile in 32 bits (the tensors are never touched)."""
+    refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27, dtype=torch.int32)), "too wide")
+    refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27 - 1, dtype=torch.int32)), "too wide")
+    refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27 - 8, dtype=torch.int32)), "must be a CUDA tensor")
