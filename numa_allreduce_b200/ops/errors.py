@@ -14,6 +14,7 @@ src/numa_all_reduce.cu:177,202.)
 
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -60,7 +61,11 @@ def reset_kernels() -> None:
     _ext.load().kernel_error_reset()
 
 
-def after_launch() -> None:
-    """Called by the op wrappers after a launch: checks under ``NAB_CHECK=1``."""
-    if check_enabled() and not torch.cuda.is_current_stream_capturing():
-        check_kernels(sync=True)
+def after_launch(device: torch.device | None = None) -> None:
+    """Called by the op wrappers after a launch: checks under ``NAB_CHECK=1``,
+    on the device of the launch (default: the current one)."""
+    if not check_enabled():
+        return
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            check_kernels(sync=True)

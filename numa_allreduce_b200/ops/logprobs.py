@@ -39,7 +39,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, v
     native = _ext.native()
     r = TokenLogprobs._make(native.token_logprobs(logits, tokens, top_k, vocab_start))
     if native.check_requested():
-        after_launch()
+        after_launch(logits.device)
     return r
 
 

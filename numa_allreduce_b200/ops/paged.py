@@ -66,7 +66,7 @@ def assign_pages(cached: torch.Tensor, block_tables: torch.Tensor, free_pages: t
     r = PageSlots._make(native.assign_pages(cached, query_start, block_tables, free_pages, taken, page_size,
                                             num_tokens))
     if native.check_requested():
-        after_launch()
+        after_launch(cached.device)
     return r
 
 
@@ -96,7 +96,7 @@ def rope_append_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
     q = native.rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
                                  interleaved, out)
     if native.check_requested():
-        after_launch()
+        after_launch(qkv.device)
     return q
 
 
@@ -122,7 +122,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         scale = 1.0 / math.sqrt(q.shape[-1])
     out = native.paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out)
     if native.check_requested():
-        after_launch()
+        after_launch(q.device)
     return out
 
 

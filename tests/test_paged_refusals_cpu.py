@@ -167,3 +167,53 @@ def test_a_table_for_more_positions_than_fit_32_bits():
     refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27, dtype=torch.int32)), "too wide")
     refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27 - 1, dtype=torch.int32)), "too wide")
     refused(lambda: attend(block_tables=torch.empty(2, 2 ** 27 - 8, dtype=torch.int32)), "must be a CUDA tensor")
+
+
+# ------------------------------------------------------ checks on request --
+def test_checks_look_at_the_tensors_device(monkeypatch):
+    """With NAB_CHECK=1 a call checks the record of the device that it ran on, whichever device is current."""
+    from numa_allreduce_b200.ops import errors, logprobs as lp, paged
+
+    seen = []
+
+    class Device:
+        def __init__(self, device):
+            seen.append(device)
+
+        def __enter__(self):
+            seen.append("in")
+
+        def __exit__(self, *a):
+            seen.append("out")
+
+    class Native:
+        def check_requested(self):
+            return True
+
+        def assign_pages(self, *a):
+            return a[:4]
+
+        def rope_append_paged(self, *a):
+            return a[0]
+
+        def paged_attention(self, *a):
+            return a[0]
+
+        def token_logprobs(self, *a):
+            return [a[0]] * 6
+
+    class OnAnotherGpu:
+        device, shape = torch.device("cuda", 3), (2, 4, 64)
+
+    monkeypatch.setenv("NAB_CHECK", "1")
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(errors, "check_kernels", lambda sync=True: seen.append("checked"))
+    for module in (lp, paged):
+        monkeypatch.setattr(module._ext, "native", Native)
+    t = OnAnotherGpu()
+    for call in (lambda: nab.assign_pages(t, t, t, t, 16), lambda: nab.rope_append_paged(t, t, t, t, t, t, t, 1),
+                 lambda: nab.paged_attention(t, t, t, t, t), lambda: nab.token_logprobs(t, t)):
+        seen.clear()
+        call()
+        assert seen == [t.device, "in", "checked", "out"]
