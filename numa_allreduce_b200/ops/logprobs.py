@@ -70,14 +70,24 @@ def join_token_logprobs(shards: Sequence[TokenLogprobs]) -> TokenLogprobs:
 def gather_token_logprobs(shard: TokenLogprobs, group=None) -> TokenLogprobs:
     """:func:`join_token_logprobs` over the ranks of a process group, each with
     its shard of the vocabulary in rank order: one all-gather of
-    ``3 + 3 top_k`` floats per row (token ids below 2^24). Every rank gets the
-    whole vocabulary's result."""
+    ``12 + 16 top_k`` bytes per row (for fp32). Every rank gets the whole
+    vocabulary's result."""
     rows, k = shard.top_logprobs.shape
-    mine = torch.cat([torch.stack([shard.logprob, shard.entropy, shard.lse], -1), shard.top_logprobs,
-                      shard.top_tokens.float(), shard.top_logits], -1)
+    dtype = shard.lse.dtype
+    # as whole numbers of the floats' width: an id keeps its bits (in one or two of them), and so does a NaN
+    word = torch.int64 if dtype == torch.float64 else torch.int32
+    fields = (torch.stack([shard.logprob, shard.entropy, shard.lse], -1), shard.top_logprobs, shard.top_logits,
+              shard.top_tokens)
+    mine = torch.cat([t.contiguous().view(word) for t in fields], -1)
     world = dist.get_world_size(group)
-    parts = torch.empty(world * rows, 3 + 3 * k, dtype=mine.dtype, device=mine.device)
-    dist.all_gather_into_tensor(parts, mine.contiguous(), group=group)
-    return join_token_logprobs([
-        TokenLogprobs(p[:, 0], p[:, 1], p[:, 2], p[:, 3:3 + k], p[:, 3 + k:3 + 2 * k].long(), p[:, 3 + 2 * k:])
-        for p in parts.view(world, rows, 3 + 3 * k)])
+    parts = torch.empty(world * rows, mine.shape[1], dtype=word, device=mine.device)
+    dist.all_gather_into_tensor(parts, mine, group=group)
+
+    def result(p: torch.Tensor) -> TokenLogprobs:
+        logprob, entropy, lse = p[:, :3].contiguous().view(dtype).unbind(-1)
+        top, raw = (p[:, 3 + i * k:3 + (i + 1) * k].contiguous().view(dtype) for i in range(2))
+        ids = torch.empty(rows, k, dtype=torch.int64, device=p.device)
+        ids.view(word).copy_(p[:, 3 + 2 * k:])
+        return TokenLogprobs(logprob, entropy, lse, top, ids, raw)
+
+    return join_token_logprobs([result(p) for p in parts.view(world, rows, mine.shape[1])])
