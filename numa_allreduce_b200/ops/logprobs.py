@@ -73,6 +73,8 @@ def gather_token_logprobs(shard: TokenLogprobs, group=None) -> TokenLogprobs:
     ``12 + 16 top_k`` bytes per row (for fp32). Every rank gets the whole
     vocabulary's result."""
     rows, k = shard.top_logprobs.shape
+    if rows == 0:
+        return shard
     dtype = shard.lse.dtype
     # as whole numbers of the floats' width: an id keeps its bits (in one or two of them), and so does a NaN
     word = torch.int64 if dtype == torch.float64 else torch.int32
