@@ -40,7 +40,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from ..ops import _ext
-from ..ops.errors import check_enabled, check_kernels
+from ..ops.errors import KernelError, check_enabled, check_kernels
 from ..ops.fused import fused_allreduce_rmsnorm, rmsnorm_residual
 from ..ops.gemm import gemm, gemm_allreduce_rmsnorm, gemm_swiglu, interleave_gate_up, pack_weight
 from ..ops.logprobs import TokenLogprobs, gather_token_logprobs, token_logprobs
@@ -107,7 +107,10 @@ class LlamaTPDecoder:
             default ``context`` for all).
         page_size: rows of a page (paged only).
         max_new: tokens per request that the pool has room for beyond
-            ``lengths`` (paged only).
+            ``lengths`` (paged only). A request that finds no page keeps its
+            length, which tells it (``paged_step.lengths``); the token is not
+            stored, nor attended to. With ``NAB_CHECK=1`` that step raises
+            :class:`~numa_allreduce_b200.KernelError`.
         logprobs: with a number, each step also leaves the new tokens'
             log-probabilities, entropies and that many top alternatives in
             ``self.logprobs`` (:class:`~numa_allreduce_b200.TokenLogprobs`).
@@ -275,6 +278,11 @@ class LlamaTPDecoder:
         if self.kv == "paged":
             paged = self.paged_step = assign_pages(self.cached, self.block_tables, self.free_pages, self.taken,
                                                    self.page_size)
+            if check_enabled() and not torch.cuda.is_current_stream_capturing():
+                short = (paged.lengths <= self.cached).nonzero().flatten().tolist()
+                if short:
+                    raise KernelError(f"no page for the new token of requests {short}: the pool has room for max_new "
+                                      "tokens per request")
         for i, L in enumerate(self.layers):
             self._proj(self.x, self._w(i, "wqkv"), self.qkv)
             attn = self.attn.view(self.B, self.Hq, cfg.head_dim)
