@@ -244,7 +244,7 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
                                    given->size(2) == D && given->is_contiguous() &&
                                    given->scalar_type() == qkv.scalar_type() && aligned16(*given)),
               op, ": out must be contiguous [", T, ", ", Hq, ", ", D, "] of qkv's type");
-  TORCH_CHECK(aligned16(qkv) && qkv.stride(0) % 8 == 0, op, ": the rows of qkv must be 16-byte aligned");
+  TORCH_CHECK(aligned16(qkv) && (T <= 1 || qkv.stride(0) % 8 == 0), op, ": the rows of qkv must be 16-byte aligned");
   TORCH_CHECK(cos.dim() == 2 && cos.is_contiguous() && sin.is_contiguous() && sin.sizes() == cos.sizes() &&
                   cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.size(0) >= 1,
               op, ": cos and sin must be contiguous float32 [positions, rotary_dim / 2]");

@@ -217,3 +217,12 @@ def test_checks_look_at_the_tensors_device(monkeypatch):
         seen.clear()
         call()
         assert seen == [t.device, "in", "checked", "out"]
+
+
+# ------------------------------------------------- what is not to be refused --
+def test_one_row_of_any_stride():
+    """The stride of a single row says nothing."""
+    refused(lambda: append(qkv=torch.zeros(512, 1, dtype=BF).t(), positions=i32(1), slots=torch.arange(1)),
+            "must be a CUDA tensor")
+    refused(lambda: append(qkv=torch.zeros(516, dtype=BF).as_strided((1, 512), (4, 1)), positions=i32(1),
+                           slots=torch.arange(1)), "must be a CUDA tensor")
