@@ -23,6 +23,7 @@
 #include <torch/torch.h>
 
 #include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <initializer_list>
 #include <optional>
@@ -226,7 +227,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
   return {positions, slots, lengths, taken_out};
 }
 
-// out: null for a new tensor
+// out: null for a new tensor (and in paged_attention: no scale for 1 / sqrt(head_dim))
 at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const at::Tensor& sin,
                                 const at::Tensor& positions, const at::Tensor& slots, at::Tensor& k_pages,
                                 at::Tensor& v_pages, int64_t q_heads, const OptTensor& q_norm, const OptTensor& k_norm,
@@ -305,7 +306,8 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
 }
 
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                              const at::Tensor& block_tables, const at::Tensor& lengths, double scale,
+                              const at::Tensor& block_tables, const at::Tensor& lengths,
+                              std::optional<double> scale,
                               const at::Tensor* given) {
   constexpr const char* op = "paged_attention";
   const int dtype = half_dtype(op, q, "q");
@@ -357,7 +359,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
   a.Hq = static_cast<int>(Hq);
   a.Hkv = static_cast<int>(Hkv);
   a.D = static_cast<int>(D);
-  a.scale = static_cast<float>(scale);
+  a.scale = static_cast<float>(scale.value_or(1.0 / std::sqrt(static_cast<double>(D))));
   // of this call alone: two streams or graphs never share it
   const at::Tensor ws = fresh({nab::paged_attention_ws_floats(a.B, a.M, a.P, a.Hq, a.Hkv, a.D, sms)}, at::kFloat, q);
   a.ws = ws.mutable_data_ptr<float>();
@@ -449,6 +451,13 @@ class Args {
     if (v == -1 && PyErr_Occurred()) refuse(name, "a 64-bit integer", o);
     return v;
   }
+  std::optional<double> optional_number(const char* name) {
+    if (args_[i_] == Py_None) {
+      ++i_;
+      return std::nullopt;
+    }
+    return number(name);
+  }
   double number(const char* name) {
     PyObject* o = args_[i_++];
     const double v = PyFloat_AsDouble(o);
@@ -528,7 +537,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Args a("paged_attention", args, n, 7);
   const at::Tensor &q = a.tensor("q"), &k_pages = a.tensor("k_pages"), &v_pages = a.tensor("v_pages");
   const at::Tensor &block_tables = a.tensor("block_tables"), &lengths = a.tensor("lengths");
-  const double scale = a.number("scale");
+  const std::optional<double> scale = a.optional_number("scale");
   const OptTensor out = a.optional_tensor("out");
   return THPVariable_Wrap(without_gil("nab::paged_attention", [&] {
     return paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out ? &*out : nullptr);

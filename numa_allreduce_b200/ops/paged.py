@@ -118,8 +118,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     requests may be mixed; parts of a request are joined in a second launch.
     """
     native = _ext.native()
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
     out = native.paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out)
     if native.check_requested():
         after_launch(q.device)

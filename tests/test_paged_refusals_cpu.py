@@ -226,3 +226,13 @@ def test_one_row_of_any_stride():
             "must be a CUDA tensor")
     refused(lambda: append(qkv=torch.zeros(516, dtype=BF).as_strided((1, 512), (4, 1)), positions=i32(1),
                            slots=torch.arange(1)), "must be a CUDA tensor")
+
+
+def test_the_default_scale_needs_no_shape():
+    """A bad q is refused with its name without a scale too."""
+    refused(lambda: attend(q=torch.zeros((), dtype=BF)), "paged_attention: q must be")
+    refused(lambda: attend(q=torch.zeros(2, 4, 0, dtype=BF)), "paged_attention: q must be")
+    with pytest.raises(TypeError, match="paged_attention: q must be a tensor, got NoneType"):
+        attend(q=None)
+    with pytest.raises(TypeError, match="paged_attention: scale must be a number, got str"):
+        attend(scale="1")
