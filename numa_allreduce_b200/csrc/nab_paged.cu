@@ -316,10 +316,10 @@ void launch_runs(cudaStream_t s, const RopeAppendDev& p) {
 }
 
 template <typename T, int D, bool kInterleaved>
-void launch_append(cudaStream_t s, const RopeAppendDev& p) {
+void launch_append(cudaStream_t s, const RopeAppendDev& p, int sms) {
   // one head per group while that fills the GPU's threads less than twice, else runs of 4
   const int64_t threads = p.a.T * (p.a.Hq + 2 * p.a.Hkv) * (D / 16);
-  if (threads <= 2 * 148 * 2048) {
+  if (threads <= int64_t{2} * sms * 2048) {
     launch_runs<T, D, kInterleaved, 1>(s, p);
   } else {
     launch_runs<T, D, kInterleaved, 4>(s, p);
@@ -327,20 +327,20 @@ void launch_append(cudaStream_t s, const RopeAppendDev& p) {
 }
 
 template <typename T>
-void dispatch_append(cudaStream_t s, const RopeAppendDev& p, bool interleaved) {
+void dispatch_append(cudaStream_t s, const RopeAppendDev& p, bool interleaved, int sms) {
   if (p.a.D == 64) {
-    interleaved ? launch_append<T, 64, true>(s, p) : launch_append<T, 64, false>(s, p);
+    interleaved ? launch_append<T, 64, true>(s, p, sms) : launch_append<T, 64, false>(s, p, sms);
   } else {
-    interleaved ? launch_append<T, 128, true>(s, p) : launch_append<T, 128, false>(s, p);
+    interleaved ? launch_append<T, 128, true>(s, p, sms) : launch_append<T, 128, false>(s, p, sms);
   }
 }
 
 }  // namespace
 
-void assign_pages(cudaStream_t s, const AssignPagesArgs& a) {
+void assign_pages(cudaStream_t s, const AssignPagesArgs& a, int sms) {
   if (a.B < 1 || a.B > kMaxPagedRequests) throw std::invalid_argument("assign_pages: 1 to 8192 requests");
   const int64_t rows = std::max({a.T, a.B, 1});
-  const int grid = static_cast<int>(std::min<int64_t>(148, (rows + kAssignThreads - 1) / kAssignThreads));
+  const int grid = static_cast<int>(std::min<int64_t>(sms, (rows + kAssignThreads - 1) / kAssignThreads));
   const size_t smem = (static_cast<size_t>(a.B) + (a.starts ? a.B + 1 : 0)) * sizeof(int);
   // The limit of 48 KB without opting in is for this and the kernel's static shared memory together. The attribute is
   // the device's and cheap: set on each such call.
@@ -350,14 +350,14 @@ void assign_pages(cudaStream_t s, const AssignPagesArgs& a) {
   launch(k_assign_pages, grid, kAssignThreads, smem, s, "assign_pages", a);
 }
 
-void rope_append_paged(cudaStream_t s, const RopeAppendArgs& a, int dtype, bool interleaved) {
+void rope_append_paged(cudaStream_t s, const RopeAppendArgs& a, int dtype, bool interleaved, int sms) {
   if (a.T == 0) return;
   const KernelErrorRecord rec = kernel_error_record();
   const RopeAppendDev p{a, rec.dev, rec.host};
   if (dtype == kF16) {
-    dispatch_append<__half>(s, p, interleaved);
+    dispatch_append<__half>(s, p, interleaved, sms);
   } else {
-    dispatch_append<__nv_bfloat16>(s, p, interleaved);
+    dispatch_append<__nv_bfloat16>(s, p, interleaved, sms);
   }
 }
 

@@ -27,7 +27,7 @@ struct AssignPagesArgs {
   int* taken_out;          // [1]
   int B, M, F, T, P;
 };
-void assign_pages(cudaStream_t s, const AssignPagesArgs& a);
+void assign_pages(cudaStream_t s, const AssignPagesArgs& a, int sms);
 
 struct RopeAppendArgs {
   const void* qkv;         // [T, (Hq + 2 Hkv) * D], row stride qkv_stride
@@ -46,7 +46,7 @@ struct RopeAppendArgs {
   float eps;
 };
 // dtype: kF16 or kBF16 (qkv, norms, pages and q_out share it).
-void rope_append_paged(cudaStream_t s, const RopeAppendArgs& a, int dtype, bool interleaved);
+void rope_append_paged(cudaStream_t s, const RopeAppendArgs& a, int dtype, bool interleaved, int sms);
 
 struct PagedAttnArgs {
   const void* q;           // [B, Hq, D], batch stride q_stride

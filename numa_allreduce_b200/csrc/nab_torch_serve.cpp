@@ -223,7 +223,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> assign_pages(const at
   a.F = static_cast<int>(free_pages.size(0));
   a.T = static_cast<int>(num_tokens);
   a.P = static_cast<int>(page_size);
-  nab::assign_pages(at::cuda::getCurrentCUDAStream().stream(), a);
+  nab::assign_pages(at::cuda::getCurrentCUDAStream().stream(), a, sms_of(cached));
   return {positions, slots, lengths, taken_out};
 }
 
@@ -301,7 +301,7 @@ at::Tensor rope_append_paged(const at::Tensor& qkv, const at::Tensor& cos, const
   a.P = static_cast<int>(P);
   a.max_pos = static_cast<int>(cos.size(0));
   a.eps = static_cast<float>(eps);
-  nab::rope_append_paged(at::cuda::getCurrentCUDAStream().stream(), a, dtype, interleaved);
+  nab::rope_append_paged(at::cuda::getCurrentCUDAStream().stream(), a, dtype, interleaved, sms_of(qkv));
   return out;
 }
 
