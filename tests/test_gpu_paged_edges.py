@@ -204,3 +204,36 @@ def test_infinite_values_stay_infinite(length, hq, dtype):
     v[tables[0, 2].item(), 0, 7, 5] = v[tables[0, 4].item(), 0, 1, 9] = 0
     want = nab.paged_attention(q, k, v, tables, torch.tensor([length], dtype=torch.int32, device="cuda"), scale=0.02)
     assert torch.equal(out[..., finite], want[..., finite])
+
+
+@pytest.mark.parametrize("hq,hkv,dtype,batch,most,form", [
+    (8, 2, BF, 7, 6000, "even"), (24, 2, FP, 7, 6000, "even"),      # few segments: descriptors by segment
+    (8, 2, BF, 160, 400, "even"), (24, 2, BF, 160, 400, "even"),    # more segments than CTAs
+    (32, 2, BF, 300, 64, "whole"), (8, 1, BF, 20, 1000, "cluster"), (24, 1, BF, 20, 1000, "cluster"),
+])
+def test_a_captured_call_replays_at_any_lengths(hq, hkv, dtype, batch, most, form):
+    """Ranges, parts and descriptors are made from the lengths that each replay finds."""
+    page, d = 16, 128
+    k, v, tables = make_cache([most] * 3, hkv, d, page, dtype, seed=batch)
+    k[k.isnan()] = 0  # every row may count: there is one length or another that reaches it
+    v[~torch.isfinite(v)] = 0
+    tables = tables[torch.arange(batch, device="cuda") % 3].contiguous()
+    q = torch.randn(batch, hq, d, generator=gen(batch), device="cuda").to(dtype)
+    n = torch.full((batch,), most, dtype=torch.int32, device="cuda")
+    nab.paged_attention(q, k, v, tables, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = nab.paged_attention(q, k, v, tables, n)
+    g = torch.Generator().manual_seed(batch)
+    some = torch.randint(0, most + 1, (batch,), generator=g)
+    cases = [torch.full((batch,), most), some, torch.zeros(batch, dtype=torch.long), torch.ones(batch, dtype=torch.long),
+             torch.where(torch.arange(batch) == batch // 2, most, 0), torch.where(some % 3 == 0, 0, some % 70),
+             torch.where(torch.arange(batch) % 2 == 0, most, 1)]
+    for lengths in cases:
+        n.copy_(lengths)
+        graph.replay()
+        check_attention(out, q, k, v, tables, lengths.tolist(), d ** -0.5)
+        assert torch.equal(out, nab.paged_attention(q, k, v, tables, n))
+    nab.check_kernels()
+    del graph
