@@ -480,14 +480,15 @@ class Args {
   Py_ssize_t i_ = 0;
 };
 
-// Runs f without the GIL, as an event that profilers see.
-template <typename F>
-auto without_gil(const char* name, F&& f) {
+// Runs f without the GIL, as an event that profilers see, with its inputs.
+template <typename F, typename... Inputs>
+auto without_gil(const char* name, F&& f, const Inputs&... inputs) {
   struct Released {
     PyThreadState* state = PyEval_SaveThread();
     ~Released() { PyEval_RestoreThread(state); }
   } released;
-  RECORD_FUNCTION(name, std::vector<c10::IValue>{});
+  const auto values = [&] { return std::vector<c10::IValue>{c10::IValue(inputs)...}; };  // made when one is listening
+  RECORD_FUNCTION(name, values());
   return f();
 }
 
@@ -510,7 +511,7 @@ PyObject* py_assign_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t page_size = a.integer("page_size"), num_tokens = a.integer("num_tokens");
   return tuple_of(without_gil("nab::assign_pages", [&] {
     return assign_pages(cached, query_start, block_tables, free_pages, taken, page_size, num_tokens);
-  }));
+  }, cached, query_start, block_tables, free_pages, taken, page_size, num_tokens));
   END_HANDLE_TH_ERRORS
 }
 
@@ -528,7 +529,7 @@ PyObject* py_rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(without_gil("nab::rope_append_paged", [&] {
     return rope_append_paged(qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps,
                              interleaved, out ? &*out : nullptr);
-  }));
+  }, qkv, cos, sin, positions, slots, k_pages, v_pages, q_heads, q_norm, k_norm, eps, interleaved, out));
   END_HANDLE_TH_ERRORS
 }
 
@@ -541,7 +542,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const OptTensor out = a.optional_tensor("out");
   return THPVariable_Wrap(without_gil("nab::paged_attention", [&] {
     return paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out ? &*out : nullptr);
-  }));
+  }, q, k_pages, v_pages, block_tables, lengths, scale, out));
   END_HANDLE_TH_ERRORS
 }
 
@@ -550,8 +551,9 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Args a("token_logprobs", args, n, 4);
   const at::Tensor &logits = a.tensor("logits"), &tokens = a.tensor("tokens");
   const int64_t top_k = a.integer("top_k"), vocab_start = a.integer("vocab_start");
-  return tuple_of(
-      without_gil("nab::token_logprobs", [&] { return token_logprobs(logits, tokens, top_k, vocab_start); }));
+  return tuple_of(without_gil("nab::token_logprobs",
+                              [&] { return token_logprobs(logits, tokens, top_k, vocab_start); }, logits, tokens, top_k,
+                              vocab_start));
   END_HANDLE_TH_ERRORS
 }
 
