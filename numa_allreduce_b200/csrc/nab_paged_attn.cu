@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kPThreads, 2)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float mn = fmaxf(m[r], mx);
-      grown |= mn != m[r];
+      grown |= mn != m[r] && m[r] != -INFINITY;  // (nothing to scale before the first score)
       // every score -inf so far: subtract 0, so that exp(-inf) = 0 and no NaN comes from inf - inf
       const float ms = mn == -INFINITY ? 0.f : mn;
       alpha[r] = ex2(m[r] - ms);
@@ -559,9 +559,9 @@ __global__ void __launch_bounds__(kPThreads, 2)
       l[r] = l[r] * alpha[r] + sum;
       // For the product with V a probability is the sum of two 16-bit values, its rounding and what that left out: off
       // by 2^-16 of it in bf16 and 2^-22 in fp16, where the rounding alone is 2^-8 and 2^-11. (The second value's sign
-      // may differ: a product of it with an infinity must not join the first's.) One value against two: up to 8 heads 64
-      // requests of up to 8192 172.5 / 173.3 us, 1 of 1025 5.75 / 5.82; 16 heads 36.9 / 38.9 for 32 of up to 2500, 7.0
-      // / 7.6 for 1 of 1025.
+      // may differ: a product of it with an infinity must not join the first's.) One value against two (us):
+      // up to 8 heads 64 requests of up to 8192 171.4 / 172.2, 640 of up to 256 19.4 / 19.9, 1 of 1025 5.95 / 6.0; 16
+      // heads 175.8 / 177.2, 32 of up to 2500 36.8 / 38.5, 1 of 1025 6.9 / 7.5.
 #pragma unroll
       for (int x = 0; x < kSteps; ++x) {
 #pragma unroll
@@ -666,8 +666,8 @@ __global__ void __launch_bounds__(kPThreads, 2)
     if (!kWide) {  // the probabilities' second values; an infinity of V stays what the first ones made of it
 #pragma unroll
       for (int j = 0; j < kNt; ++j) {
-        acc[j][0] += fabsf(acc[j][0]) < INFINITY ? acc[j][2] : 0.f;
-        acc[j][1] += fabsf(acc[j][1]) < INFINITY ? acc[j][3] : 0.f;
+        if (fabsf(acc[j][0]) < INFINITY) acc[j][0] += acc[j][2];
+        if (fabsf(acc[j][1]) < INFINITY) acc[j][1] += acc[j][3];
       }
     }
 #pragma unroll
