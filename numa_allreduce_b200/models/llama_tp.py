@@ -314,11 +314,11 @@ class LlamaTPDecoder:
         logits = self.logits[:, :self.v_valid]
         if self.v_valid > 0:
             val, idx = logits.float().max(dim=-1)
-            idx = idx + self.v_start
         else:  # a shard of padding alone: token 0 at -inf
             val, idx = self.logits.new_full((self.B,), -math.inf, dtype=torch.float32), torch.zeros_like(self.tokens)
         if self.world > 1:
-            mine = torch.stack([val, idx.float()], dim=-1).reshape(-1)
+            ids = idx + self.v_start if self.v_valid > 0 else idx
+            mine = torch.stack([val, ids.float()], dim=-1).reshape(-1)
             dist.all_gather_into_tensor(self._gathered, mine)
             allv = self._gathered.view(self.world, self.B, 2)
             best = allv[:, :, 0].argmax(dim=0)
