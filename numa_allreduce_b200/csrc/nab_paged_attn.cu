@@ -7,7 +7,7 @@
 // operations a byte. The contractions are warp-level 16-bit MMAs (m16n8k16,
 // fp32 accumulators): rows are the query heads of one kv head, so one
 // operand pass serves up to 16 heads, and the probabilities stay in registers
-// between the two products. A tcgen05 version needs them in shared memory
+// between the two products, as two 16-bit values each. A tcgen05 version needs them in shared memory
 // and two TMEM round trips with CTA barriers per chunk (the contiguous-cache
 // kernel of nab_attn_sm100.cu), a serial chain that costs more than the
 // bytes of a chunk; here four warps stream independently.
@@ -1003,14 +1003,15 @@ PagedPlan plan_of(int B, int M, int P, int Hq, int Hkv, int D, int sms) {
     throw std::invalid_argument("paged_attention: too many positions for one call");
   // The cluster form takes ceil(tiles / c) tiles one after the other, the even one ceil(tiles * segments / slots) and
   // about three more for its second launch. Measured (us, cluster / even; 8 heads per kv head, D = 128): 1 request of
-  // 1025 6.2 / 7.0, of 4096 9.9 / 7.5; 32 of 2500 12.1 / 13.8, of 1 to 2500 9.6 / 11.6; 128 of 1025 16.6 / 18.6. The
+  // 1025 6.0 / 7.1, of 4096 9.9 / 7.6; 32 of 2500 12.1 / 14.0, of 1 to 2500 9.7 / 12.2; 128 of 1025 16.8 / 19.1. The
   // bound of 10 tiles keeps ragged batches, where the longest request decides, from losing more than that.
   int c = 1;
   while (c < kMaxCluster && 2 * c <= tiles && segments * c * 2 <= slots) c *= 2;
   const int64_t share = (tiles + c - 1) / c, even = (tiles * segments + slots - 1) / slots;
   p.cluster = segments * c <= slots && share <= std::min<int64_t>(10, even + 3) ? c : 0;
   // Short requests are not worth a cut: up to 4 tiles of imbalance against the second launch (whole / even: 640 of up
-  // to 256 positions 15.9 / 17.0 us, 160 of up to 5 with 4 kv heads 7.7 / 8.7).
+  // to 256 positions in pages of 64 16.7 / 17.2 us, in pages of 16, whose boxes take longer to issue, 19.3 / 17.1; 160
+  // of up to 5 with 4 kv heads 7.3 / 8.5).
   p.whole = !p.cluster && tiles <= 4;
   p.grid = static_cast<int>(p.cluster ? segments * c : std::min<int64_t>(slots, p.whole ? segments : tiles * segments));
   // parts of a segment when all requests are of one length: grid / segments and two ends

@@ -12,7 +12,11 @@ from .errors import after_launch
 
 
 class TokenLogprobs(NamedTuple):
-    """What :func:`token_logprobs` gives for each row of logits (fp32, token ids int64)."""
+    """What :func:`token_logprobs` gives for each row of logits (fp32, token ids int64).
+
+    All of it lies in one allocation, which lives as long as any part: clone
+    what is to be kept alone.
+    """
 
     logprob: torch.Tensor       # [rows]: of the given token, -inf if it is not in this part of the vocabulary
     entropy: torch.Tensor       # [rows]: of the distribution, in nats
@@ -25,8 +29,11 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, vocab_start: int = 0) -> TokenLogprobs:
     """Log-softmax of ``logits[rows, vocabulary]`` at ``tokens``, and its entropy and ``top_k`` largest entries.
 
-    One launch that reads the logits (fp32, fp16 or bf16; rows may be further
-    apart than the vocabulary) once; sums in fp32. ``top_k`` is at most 32;
+    One launch and one pass over the logits (fp32, fp16 or bf16; rows may be
+    further apart than the vocabulary), sums in fp32. The few parts of a row
+    that can hold its largest entries are read again for them, and a row whose
+    maximum is above 2^24 or below -2^23 (fp16: below -50000) is summed again.
+    ``top_k`` is at most 32;
     equal logits rank by the lowest token id. Entries of -inf (masked tokens)
     have probability 0. A row that holds NaN or +inf, or only -inf, gives NaN
     (``lse`` of the last is -inf); NaN ranks as -inf.
@@ -34,7 +41,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, v
     ``logits`` may be one shard of the vocabulary, with column 0 the token
     ``vocab_start``: the result is that of the shard alone, and
     :func:`join_token_logprobs` makes the whole vocabulary's from all shards.
-    For inference: logits that require a gradient are refused.
+    For inference: logits that require a gradient, or carry a forward-mode
+    tangent, are refused, and so are tensors that are not plain memory (fake,
+    batched or wrapped ones).
     """
     native = _ext.native()
     r = TokenLogprobs._make(native.token_logprobs(logits, tokens, top_k, vocab_start))

@@ -15,7 +15,11 @@ requests have different lengths is::
 
 Lengths, tables and the free list are read on the device: nothing
 synchronises, and a captured CUDA graph replays at any lengths. The operators
-are for inference: a tensor that requires a gradient is refused.
+are for inference: a tensor that requires a gradient, or carries a
+forward-mode tangent, is refused. They are functions of the extension module
+and not ``torch.ops``: dispatch modes, ``torch.export`` and the like do not see
+them, and fake, batched or wrapped tensors are refused. A tensor that a call
+writes must not share memory with another one of the call.
 """
 
 from __future__ import annotations
@@ -30,7 +34,11 @@ from .errors import after_launch
 
 
 class PageSlots(NamedTuple):
-    """What :func:`assign_pages` gives for one step."""
+    """What :func:`assign_pages` gives for one step.
+
+    All four lie in one allocation, which lives as long as any of them: clone
+    what is to be kept when the slots of a long prompt are not.
+    """
 
     positions: torch.Tensor  # int32 [tokens]: position in its request
     slots: torch.Tensor      # int64 [tokens]: slot in the cache, -1 where there is none
@@ -53,7 +61,8 @@ def assign_pages(cached: torch.Tensor, block_tables: torch.Tensor, free_pages: t
 
     ``num_tokens`` is the number of rows (needed with ``query_start``): rows
     past the last request's, the padding of a batch, get position 0 and slot
-    -1. Where the free list or the table's width runs out, tokens get slot -1
+    -1. Tokens past ``num_tokens`` get their pages and count in ``lengths``,
+    but no position and slot: append them before attending. Where the free list or the table's width runs out, tokens get slot -1
     and the table -1, and ``lengths`` counts only positions that have a page:
     ``lengths[b] < cached[b] + new tokens`` tells it. ``cached`` and ``taken``
     are not changed.
@@ -108,14 +117,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q`` is ``[requests, q_heads, head_dim]`` (consecutive query heads share a
     kv head; rows may be further apart), ``lengths[b]`` the positions that
     request ``b`` attends to, the new token's own among them (append it
-    first). ``scale`` defaults to ``1 / sqrt(head_dim)``. A request of length
+    first). ``scale`` defaults to ``1 / sqrt(head_dim)``. Scores, softmax and
+    sums are in fp32 (a probability enters its product with v as two 16-bit
+    values), with one rounding at the end. A request of length
     0 gives zeros; rows of its pages past a request's length are never used,
     whatever they hold. A length past the table's width is cut to it, and a
     page id outside the cache reads as zeros; both are recorded
     (:func:`~numa_allreduce_b200.check_kernels`).
 
-    The work of all requests is split evenly over the GPU, so long and short
-    requests may be mixed; parts of a request are joined in a second launch.
+    Long and short requests may be mixed. The width of the table, which bounds
+    the lengths, decides how the work is dealt out: a cluster of CTAs per
+    request and kv head for few or short ones; whole requests for many short
+    ones; otherwise all positions split evenly over the GPU, and the parts of a
+    request joined in a second launch. A table no wider than the step
+    needs is the fastest.
     """
     native = _ext.native()
     out = native.paged_attention(q, k_pages, v_pages, block_tables, lengths, scale, out)
